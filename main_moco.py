@@ -6,7 +6,8 @@ at reference main_moco.py:38-101; launch skeleton :103-134, worker :137-287).
 MoCo v2 = --mlp --moco-t 0.2 --aug-plus --cos.
 
 Extra flags vs the reference: --data synthetic (no-network environments),
---device {cuda,cpu}, --moco-dtype {fp32,bf16}, --synthetic-len, --load-size.
+--device {cuda,cpu}, --moco-dtype {fp32,bf16}, --synthetic-len, --load-size,
+--optimizer {sgd,adamw,adamw8bit}, --clip-grad.
 """
 
 import argparse
@@ -25,7 +26,7 @@ import moco_amd
 from moco_amd.engine import MoCoStepper, train_epoch
 from moco_amd.loader import build_dataset
 from moco_amd.models.resnet import MODEL_REGISTRY, build_model
-from moco_amd.ops import FusedSGD
+from moco_amd.ops import FusedAdamW, FusedSGD
 from moco_amd.utils import adjust_learning_rate, save_checkpoint
 
 model_names = sorted(MODEL_REGISTRY)
@@ -47,6 +48,12 @@ def get_parser():
     parser.add_argument("--momentum", default=0.9, type=float)
     parser.add_argument("--wd", "--weight-decay", default=1e-4, type=float,
                         dest="weight_decay")
+    parser.add_argument("--optimizer", default="sgd",
+                        choices=["sgd", "adamw", "adamw8bit"],
+                        help="adamw8bit keeps AdamW's moments in 8 bits; "
+                             "--momentum is SGD's (AdamW: betas 0.9, 0.999)")
+    parser.add_argument("--clip-grad", default=None, type=float,
+                        help="AdamW: clip the gradients' global norm to this")
     parser.add_argument("-p", "--print-freq", default=10, type=int)
     parser.add_argument("--resume", default="", type=str)
     parser.add_argument("--world-size", default=-1, type=int)
@@ -93,7 +100,10 @@ def get_parser():
 
 
 def main(argv=None):
-    args = get_parser().parse_args(argv)
+    parser = get_parser()
+    args = parser.parse_args(argv)
+    if args.clip_grad is not None and args.optimizer == "sgd":
+        parser.error("--clip-grad needs --optimizer adamw or adamw8bit")
 
     if args.debug_serialize:
         # must be set before the first HIP call in every worker
@@ -176,9 +186,15 @@ def main_worker(gpu, ngpus_per_node, args):
             ddp_kwargs["device_ids"] = [device.index]
         model = torch.nn.parallel.DistributedDataParallel(model, **ddp_kwargs)
 
-    optimizer = FusedSGD(model.parameters(), args.lr,
-                         momentum=args.momentum,
-                         weight_decay=args.weight_decay)
+    if args.optimizer == "sgd":
+        optimizer = FusedSGD(model.parameters(), args.lr,
+                             momentum=args.momentum,
+                             weight_decay=args.weight_decay)
+    else:
+        optimizer = FusedAdamW(
+            model.parameters(), args.lr, weight_decay=args.weight_decay,
+            state_bits=8 if args.optimizer == "adamw8bit" else 32,
+            max_grad_norm=args.clip_grad, seed=seed)
 
     if args.resume:
         if os.path.isfile(args.resume):

@@ -71,6 +71,13 @@ from .functional import (  # noqa: E402
     softmax_ce_label0,
 )
 from .multi_tensor import FusedSGD, MultiTensorEMA  # noqa: E402
+from .adamw import (  # noqa: E402
+    FusedAdamW,
+    adamw8bit_,
+    adamw8bit_values,
+    adamw_,
+    grad_norm,
+)
 from .augment import two_crop_augment  # noqa: E402
 
 __all__ = [
@@ -84,5 +91,10 @@ __all__ = [
     "ema_update_",
     "MultiTensorEMA",
     "FusedSGD",
+    "FusedAdamW",
+    "adamw_",
+    "adamw8bit_",
+    "adamw8bit_values",
+    "grad_norm",
     "two_crop_augment",
 ]

@@ -6,6 +6,9 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "hip/launchers.h"
 
 namespace {
@@ -236,6 +239,275 @@ void ema_flat(torch::Tensor dst, torch::Tensor src, double m) {
   CHECK_LAUNCH(launch_ema_flat(cur_stream(), dst.data_ptr<float>(),
                                src.data_ptr<float>(), dst.numel(),
                                (float)m));
+}
+
+// ---------------------------------------------------------------------------
+// AdamW and the gradient norm over lists of tensors (adamw.hip)
+
+using TensorList = std::vector<torch::Tensor>;
+
+int adamw_dtype(const torch::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return 0;
+    case torch::kBFloat16: return 1;
+    case torch::kHalf: return 2;
+    default: break;
+  }
+  TORCH_CHECK_TYPE(false, what, " must be float32, bfloat16 or float16, got ",
+                   t.scalar_type());
+}
+
+// same shape and same place of every element (strides of length-1 dims say
+// nothing), without gaps
+bool same_dense_layout(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.sizes() != b.sizes()) return false;
+  if (!a.is_non_overlapping_and_dense() || !b.is_non_overlapping_and_dense())
+    return false;
+  if (a.strides() == b.strides()) return true;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
+// [begin, end) in memory that a launch writes or reads
+struct Range {
+  uintptr_t begin, end;
+  bool write;
+};
+
+void add_range(std::vector<Range>& r, const torch::Tensor& t, bool write) {
+  const uintptr_t a = (uintptr_t)t.const_data_ptr();
+  r.push_back({a, a + t.numel() * t.element_size(), write});
+}
+
+// What one workgroup writes no other may touch: a tensor given twice, or two
+// views of the same memory, would be a race.
+void check_disjoint(std::vector<Range>& r) {
+  std::sort(r.begin(), r.end(),
+            [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  uintptr_t wrote = 0, read = 0;
+  for (const auto& x : r) {
+    TORCH_CHECK_VALUE(x.begin >= wrote && !(x.write && x.begin < read),
+                      "the tensors of one call must not share memory");
+    (x.write ? wrote : read) = std::max(x.write ? wrote : read, x.end);
+  }
+}
+
+// fills tables of one dtype and hands each to `launch`
+template <typename F>
+struct TableFiller {
+  AdamwTable tab;
+  F launch;
+  explicit TableFiller(F f) : launch(f) { tab.count = 0, tab.chunks = 0; }
+  void add(void* p, const void* g, void* m, void* v, void* s, int64_t n,
+           uint32_t key) {
+    const int64_t chunks = (n + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
+    TORCH_CHECK_VALUE(chunks < (int64_t)1 << 30, "a tensor of ", n,
+                      " elements is too large");
+    if (tab.count == ADAMW_TENSORS ||
+        (int64_t)tab.chunks + chunks > (int64_t)1 << 30)
+      flush();
+    const int i = tab.count++;
+    tab.p[i] = p, tab.g[i] = g, tab.m[i] = m, tab.v[i] = v, tab.s[i] = s;
+    tab.n[i] = n, tab.first[i] = tab.chunks, tab.key[i] = key;
+    tab.chunks += (uint32_t)chunks;
+  }
+  void flush() {
+    if (tab.count) launch(tab);
+    tab.count = 0, tab.chunks = 0;
+  }
+};
+
+// 2-norm over all elements of a list; every tensor dense, on one device
+torch::Tensor grad_norm_checked(const TensorList& grads) {
+  auto opts = grads[0].options().dtype(torch::kFloat32).layout(torch::kStrided);
+  auto out = torch::empty({}, opts);
+  constexpr int BLOCKS = 1024;
+  // a launch takes ADAMW_TENSORS tensors of one dtype: at most this many
+  const int64_t launches = (int64_t)grads.size() / ADAMW_TENSORS + 3;
+  auto partial = torch::empty({launches * BLOCKS},
+                              opts.dtype(torch::kFloat64));
+  double* at = partial.data_ptr<double>();
+  int used = 0;
+  for (int dtype = 0; dtype < 3; ++dtype) {
+    auto go = [&](const AdamwTable& tab) {
+      const int blocks = (int)std::min<uint32_t>(BLOCKS, tab.chunks);
+      TORCH_CHECK(used + blocks <= partial.numel());
+      CHECK_LAUNCH(launch_sumsq(cur_stream(), &tab, dtype, at + used, blocks));
+      used += blocks;
+    };
+    TableFiller<decltype(go)> fill(go);
+    for (const auto& g : grads)
+      if (g.numel() && adamw_dtype(g, "gradients") == dtype)
+        fill.add(nullptr, g.const_data_ptr(), nullptr, nullptr, nullptr,
+                 g.numel(), 0);
+    fill.flush();
+  }
+  CHECK_LAUNCH(launch_norm_final(cur_stream(), at, used,
+                                 out.data_ptr<float>()));
+  return out;
+}
+
+torch::Tensor grad_norm(const TensorList& grads) {
+  TORCH_CHECK_VALUE(!grads.empty(), "grad_norm needs at least one tensor");
+  at::cuda::CUDAGuard guard(grads[0].device());
+  TensorList dense;
+  for (const auto& g : grads) {
+    TORCH_CHECK_VALUE(g.device() == grads[0].device() && g.is_cuda(),
+                      "gradients must be on one device");
+    TORCH_CHECK_VALUE(g.layout() == torch::kStrided,
+                      "sparse gradients are not supported");
+    adamw_dtype(g, "gradients");
+    // an expanded or gapped view is laid out first: each element counts once
+    // per place that it has in the tensor
+    dense.push_back(g.is_non_overlapping_and_dense() ? g : g.contiguous());
+  }
+  return grad_norm_checked(dense);
+}
+
+// One AdamW step (8-bit moments where `scales` is not empty).  Returns the
+// gradient norm that the clip went by, if there was one.
+c10::optional<torch::Tensor> adamw_step(
+    const TensorList& params, const TensorList& grads, const TensorList& ms,
+    const TensorList& vs, const TensorList& scales, bool eight, int64_t step,
+    double lr, double beta1, double beta2, double eps, double weight_decay,
+    c10::optional<double> max_norm, c10::optional<torch::Tensor> total_norm,
+    int64_t seed) {
+  const size_t n = params.size();
+  TORCH_CHECK_VALUE(grads.size() == n && ms.size() == n && vs.size() == n &&
+                        scales.size() == (eight ? n : 0),
+                    "the lists of tensors differ in length");
+  if (n == 0) return total_norm;
+  const auto device = params[0].device();
+  at::cuda::CUDAGuard guard(device);
+  std::vector<Range> ranges;
+  ranges.reserve(5 * n);
+  const auto m_type = eight ? torch::kFloat8_e4m3fn : torch::kFloat32;
+  const auto v_type = eight ? torch::kUInt8 : torch::kFloat32;
+  bool seen[3] = {false, false, false};
+  for (size_t i = 0; i < n; ++i) {
+    const auto &p = params[i], &g = grads[i], &m = ms[i], &v = vs[i];
+    seen[adamw_dtype(p, "params")] = true;
+    TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "gradient ", i,
+                     " is ", g.scalar_type(), ", its parameter ",
+                     p.scalar_type());
+    TORCH_CHECK_VALUE(g.layout() == torch::kStrided,
+                      "sparse gradients are not supported");
+    TORCH_CHECK_TYPE(m.scalar_type() == m_type && v.scalar_type() == v_type,
+                     "the moments must be ", m_type, " and ", v_type);
+    TORCH_CHECK_VALUE(p.device() == device && g.device() == device &&
+                          m.device() == device && v.device() == device,
+                      "all tensors must be on one device");
+    TORCH_CHECK_VALUE(same_dense_layout(p, g) && same_dense_layout(p, m) &&
+                          same_dense_layout(p, v),
+                      "parameter ", i, ", its gradient and its moments must "
+                      "be dense and laid out alike");
+    add_range(ranges, p, true);
+    add_range(ranges, g, false);
+    add_range(ranges, m, true);
+    add_range(ranges, v, true);
+    if (eight) {
+      const auto& s = scales[i];
+      TORCH_CHECK_VALUE(
+          s.device() == device && s.scalar_type() == torch::kFloat32 &&
+              s.is_contiguous() && s.dim() == 2 &&
+              s.size(0) == (p.numel() + 255) / 256 && s.size(1) == 2,
+          "scales of parameter ", i, " must be contiguous float32 [",
+          (p.numel() + 255) / 256, ", 2]");
+      TORCH_CHECK_VALUE((uintptr_t)s.const_data_ptr() % 8 == 0,
+                        "scales must be aligned to 8 bytes");
+      add_range(ranges, s, true);
+    }
+  }
+  check_disjoint(ranges);
+  const float* norm = nullptr;
+  if (max_norm.has_value()) {
+    if (!total_norm.has_value()) total_norm = grad_norm_checked(grads);
+    TORCH_CHECK_VALUE(total_norm->device() == device &&
+                          total_norm->numel() == 1 &&
+                          total_norm->scalar_type() == torch::kFloat32,
+                      "total_norm must be one float32 on the tensors' device");
+    norm = total_norm->const_data_ptr<float>();
+  }
+  AdamwScalars h;
+  h.beta1 = (float)beta1;
+  h.one_minus_beta1 = (float)(1.0 - beta1);
+  h.beta2 = (float)beta2;
+  h.one_minus_beta2 = (float)(1.0 - beta2);
+  h.inv_root_bc2 =
+      (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+  h.eps = (float)eps;
+  h.decay = (float)(1.0 - lr * weight_decay);
+  h.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+  h.max_norm = (float)max_norm.value_or(0.0);
+  const uint32_t key =
+      (uint32_t)seed * 0x6A09E667u + (uint32_t)step * 0xA54FF53Au;
+  for (int dtype = 0; dtype < 3; ++dtype) {
+    if (!seen[dtype]) continue;
+    auto go = [&](const AdamwTable& tab) {
+      if (eight)
+        CHECK_LAUNCH(launch_adamw8(cur_stream(), &tab, &h, norm, dtype, key));
+      else
+        CHECK_LAUNCH(launch_adamw(cur_stream(), &tab, &h, norm, dtype));
+    };
+    TableFiller<decltype(go)> fill(go);
+    for (size_t i = 0; i < n; ++i)
+      if (params[i].numel() && adamw_dtype(params[i], "params") == dtype)
+        fill.add(params[i].data_ptr(), grads[i].const_data_ptr(),
+                 ms[i].data_ptr(), vs[i].data_ptr(),
+                 eight ? scales[i].data_ptr() : nullptr, params[i].numel(),
+                 (uint32_t)i * 0x3C6EF372u);
+    fill.flush();
+  }
+  return total_norm;
+}
+
+// decoded moments of 8-bit codes
+std::vector<TensorList> adamw8bit_values(const TensorList& ms,
+                                         const TensorList& vs,
+                                         const TensorList& scales,
+                                         torch::ScalarType dtype) {
+  TORCH_CHECK_VALUE(vs.size() == ms.size() && scales.size() == ms.size(),
+                    "the lists of tensors differ in length");
+  std::vector<TensorList> out(2);
+  if (ms.empty()) return out;
+  at::cuda::CUDAGuard guard(ms[0].device());
+  int kind = 0;
+  auto go = [&](const AdamwTable& tab) {
+    CHECK_LAUNCH(launch_adamw8_values(cur_stream(), &tab, kind));
+  };
+  TableFiller<decltype(go)> fill(go);
+  for (size_t i = 0; i < ms.size(); ++i) {
+    const auto &m = ms[i], &v = vs[i], &s = scales[i];
+    TORCH_CHECK_TYPE(m.scalar_type() == torch::kFloat8_e4m3fn &&
+                         v.scalar_type() == torch::kUInt8,
+                     "the codes must be float8_e4m3fn and uint8");
+    TORCH_CHECK_VALUE(m.device() == ms[0].device() &&
+                          v.device() == ms[0].device() &&
+                          s.device() == ms[0].device(),
+                      "all tensors must be on one device");
+    TORCH_CHECK_VALUE(same_dense_layout(m, v),
+                      "codes ", i, " must be dense and laid out alike");
+    TORCH_CHECK_VALUE(s.scalar_type() == torch::kFloat32 &&
+                          s.is_contiguous() && s.dim() == 2 &&
+                          s.size(0) == (m.numel() + 255) / 256 &&
+                          s.size(1) == 2 &&
+                          (uintptr_t)s.const_data_ptr() % 8 == 0,
+                      "scales ", i, " must be contiguous float32 [",
+                      (m.numel() + 255) / 256, ", 2], aligned to 8 bytes");
+    auto om = torch::empty_strided(m.sizes(), m.strides(),
+                                   m.options().dtype(dtype));
+    auto ov = torch::empty_strided(m.sizes(), m.strides(),
+                                   m.options().dtype(dtype));
+    kind = adamw_dtype(om, "values");
+    if (m.numel())
+      fill.add(om.data_ptr(), ov.data_ptr(), m.data_ptr(), v.data_ptr(),
+               s.data_ptr(), m.numel(), 0);
+    out[0].push_back(om);
+    out[1].push_back(ov);
+  }
+  fill.flush();
+  return out;
 }
 
 // ---------------------------------------------------------------------------
@@ -713,6 +985,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("multi_transpose_bf16", &multi_transpose_bf16);
   mod.def("multi_tensor_sgd", &multi_tensor_sgd);
   mod.def("ema_flat", &ema_flat);
+  mod.def("grad_norm", &grad_norm);
+  mod.def("adamw_step", &adamw_step);
+  mod.def("adamw8bit_values", [](const TensorList& m, const TensorList& v,
+                                 const TensorList& s, py::object dtype) {
+    return adamw8bit_values(
+        m, v, s, torch::python::detail::py_object_to_dtype(dtype));
+  });
   mod.def("two_crop_augment", &two_crop_augment);
   mod.def("bn_fwd_train", &bn_fwd_train);
   mod.def("bn_fwd_eval", &bn_fwd_eval);

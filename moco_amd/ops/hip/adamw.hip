@@ -1,0 +1,469 @@
+// AdamW over many tensors, the gradient norm over many tensors, and the
+// 8-bit form of AdamW's moments.  Beside the SGD/EMA kernels of
+// multi_tensor.hip, but with the tensor table in the kernel's arguments: no
+// device-side table is built, so nothing is kept from one call to the next.
+//
+//   g  = coef * grad              coef = min(1, max_norm / (norm + 1e-6))
+//   m' = b1 m + (1 - b1) g        v' = b2 v + (1 - b2) g^2
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// Each operation is rounded by itself (no contraction into fma): a plain
+// elementwise program in 32 bits then computes the same values, and what is
+// rounded to 8 bits afterwards falls on the same codes.
+#include "common.h"
+#include "launchers.h"
+
+#pragma clang fp contract(off)
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int CHUNK = ADAMW_CHUNK;  // elements of one table chunk
+constexpr int QBLOCK = 256;         // elements that share a pair of scales
+constexpr float TINY = 1e-30f;      // least block maximum a scale stands for
+constexpr float TOP_M = 448.f;      // largest e4m3 value
+constexpr float TOP_R = 1.9375f;    // largest value of a code of sqrt(v)
+static_assert(ADAMW_TENSORS == WAVE, "a wave looks up one tensor a lane");
+static_assert(CHUNK == THREADS * 16, "a thread handles 16 elements");
+
+// The tensor of chunk c: first[] ascends, so it is the last one whose first
+// chunk is not behind c.  One lane looks at each tensor.
+__device__ __forceinline__ int find_tensor(const uint32_t* first, int count,
+                                           uint32_t c) {
+  const int lane = threadIdx.x % WAVE;
+  const bool before = lane < count && first[lane] <= c;
+  return __popcll(__ballot(before)) - 1;
+}
+
+// V elements of type T as floats.  Tensors may be views that begin anywhere:
+// only the element's own alignment is assumed.
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float (&out)[V]) {
+  T raw[V];
+  __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = (float)raw[i];
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const float (&in)[V]) {
+  T raw[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) raw[i] = (T)in[i];  // to nearest even
+  __builtin_memcpy(p, raw, sizeof(raw));
+}
+
+// the first `n` of them (n may be <= 0); zeros behind
+template <typename T, int V>
+__device__ __forceinline__ void load_part(const T* p, float (&out)[V],
+                                          int64_t n) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = i < n ? (float)p[i] : 0.f;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_part(T* p, const float (&in)[V],
+                                           int64_t n) {
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < n) p[i] = (T)in[i];
+}
+
+// min(1, max_norm / (norm + 1e-6)); a NaN norm stays a NaN
+__device__ __forceinline__ float clip_coef(const float* norm,
+                                           float max_norm) {
+  if (norm == nullptr) return 1.f;
+  const float c = max_norm / (*norm + 1e-6f);
+  return c > 1.f ? 1.f : c;
+}
+
+// one element; r is sqrt(v')
+__device__ __forceinline__ void adamw_element(const AdamwScalars& h,
+                                              float coef, float g, float& p,
+                                              float& m, float& v, float& r) {
+  g = g * coef;
+  m = m * h.beta1 + g * h.one_minus_beta1;
+  v = v * h.beta2 + (g * g) * h.one_minus_beta2;
+  r = __fsqrt_rn(v);
+  const float q = __fdiv_rn(m, r * h.inv_root_bc2 + h.eps);
+  p = p * h.decay - q * h.step_size;
+}
+
+// 28 bytes an fp32 element (22 a 16-bit one) and some 30 operations: bound
+// by memory.  All loads of a chunk are issued before the first is used.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void adamw_kernel(
+    const AdamwTable tab, const AdamwScalars h, const float* norm) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int NV = CHUNK / (THREADS * V);
+  const int t = find_tensor(tab.first, tab.count, blockIdx.x);
+  const int64_t at = (int64_t)(blockIdx.x - tab.first[t]) * CHUNK;
+  T* p = (T*)tab.p[t] + at;
+  const T* g = (const T*)tab.g[t] + at;
+  float* m = (float*)tab.m[t] + at;
+  float* v = (float*)tab.v[t] + at;
+  const int64_t left = tab.n[t] - at;
+  const float coef = clip_coef(norm, h.max_norm);
+  float gf[NV][V], pf[NV][V], mf[NV][V], vf[NV][V], r;
+  const int i0 = threadIdx.x * V;
+  if (left >= CHUNK) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = i0 + j * THREADS * V;
+      load_vec(g + i, gf[j]);
+      load_vec(p + i, pf[j]);
+      load_vec(m + i, mf[j]);
+      load_vec(v + i, vf[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = i0 + j * THREADS * V;
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        adamw_element(h, coef, gf[j][k], pf[j][k], mf[j][k], vf[j][k], r);
+      store_vec(p + i, pf[j]);
+      store_vec(m + i, mf[j]);
+      store_vec(v + i, vf[j]);
+    }
+  } else {
+    for (int i = i0; i < left; i += THREADS * V) {
+      const int64_t n = left - i;
+      load_part(g + i, gf[0], n);
+      load_part(p + i, pf[0], n);
+      load_part(m + i, mf[0], n);
+      load_part(v + i, vf[0], n);
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        adamw_element(h, coef, gf[0][k], pf[0][k], mf[0][k], vf[0][k], r);
+      store_part(p + i, pf[0], n);
+      store_part(m + i, mf[0], n);
+      store_part(v + i, vf[0], n);
+    }
+  }
+}
+
+// ---- 8-bit moments ---------------------------------------------------------
+// m: an e4m3 code times the block's scale (its largest |m| / 448), rounded
+// to nearest; b1 = 0.9 moves m by whole steps.
+// v: kept as sqrt(v), which has half the octaves: an unsigned code of 4
+// exponent and 4 fraction bits, value 2^(e-15) (1 + f/16) (e = 0: 2^-14
+// f/16), times the block's scale (its largest root / 1.9375).  19 octaves,
+// 38 of v.  Rounded stochastically: b2 = 0.999 moves sqrt(v) by 0.05% a
+// step where codes are 3 to 6% apart, so rounding to nearest would hold it
+// still.  A value above zero keeps a code above zero, since m / (sqrt(v) +
+// eps) has no bound where v is lost and m is not.
+
+__device__ __forceinline__ float decode_root(uint32_t code) {
+  return __uint_as_float(code << 19) * 0x1p112f;
+}
+
+__device__ __forceinline__ uint32_t encode_root(float q, uint32_t dither) {
+  const uint32_t c = (__float_as_uint(q * 0x1p-112f) + dither) >> 19;
+  return q > 0.f ? min(max(c, 1u), 255u) : 0u;
+}
+
+// 19 random bits of one element: a multiplicative hash of its counter (the
+// golden ratio's and sqrt(3)'s fractions as odd multipliers), folded twice
+__device__ __forceinline__ uint32_t dither19(uint32_t x) {
+  x *= 0x9E3779B9u;
+  x ^= x >> 15;
+  x *= 0xBB67AE85u;
+  x ^= x >> 16;
+  return x >> 13;
+}
+
+// Largest of 16 neighbouring lanes.  On the bits of non-negative floats, so
+// that a NaN is larger than every number and reaches the scale.
+__device__ __forceinline__ uint32_t max16(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));
+  x = max(x,
+          (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true));
+  x = max(x,
+          (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xF, 0xF, true));
+  return x;
+}
+
+__device__ __forceinline__ void decode8(const uint2 mc, const uint2 vc,
+                                        float (&m)[8], float (&r)[8]) {
+  const uint32_t mw[2] = {mc.x, mc.y}, vw[2] = {vc.x, vc.y};
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) {
+    const auto f = (k & 2)
+        ? __builtin_amdgcn_cvt_pk_f32_fp8(mw[k / 4], true)
+        : __builtin_amdgcn_cvt_pk_f32_fp8(mw[k / 4], false);
+    m[k] = f[0];
+    m[k + 1] = f[1];
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    r[k] = decode_root((vw[k / 4] >> (8 * (k % 4))) & 255u);
+}
+
+__device__ __forceinline__ uint2 pack_m(const float (&q)[8]) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 8; k += 4) {
+    int x = __builtin_amdgcn_cvt_pk_fp8_f32(q[k], q[k + 1], 0, false);
+    w[k / 4] = __builtin_amdgcn_cvt_pk_fp8_f32(q[k + 2], q[k + 3], x, true);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// bytes [0, n) of a code word, zeros behind
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int64_t n) {
+  uint2 w = make_uint2(0, 0);
+  if (n >= 8) {
+    __builtin_memcpy(&w, p, 8);
+  } else {
+    for (int k = 0; k < n; ++k) {
+      const uint32_t b = p[k];
+      if (k < 4) w.x |= b << (8 * k);
+      else w.y |= b << (8 * (k - 4));
+    }
+  }
+  return w;
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* p, uint2 w, int64_t n) {
+  if (n >= 8) {
+    __builtin_memcpy(p, &w, 8);
+  } else {
+    for (int k = 0; k < n; ++k)
+      p[k] = (uint8_t)((k < 4 ? w.x >> (8 * k) : w.y >> (8 * (k - 4))));
+  }
+}
+
+// 16 lanes share a block of 256 elements: lane l holds elements l*8.. of
+// each half, so that a wave reads whole lines and the block's maximum needs
+// no shared memory (four DPP steps).
+template <typename T>
+__global__ __launch_bounds__(THREADS) void adamw8_kernel(
+    const AdamwTable tab, const AdamwScalars h, const float* norm,
+    uint32_t seed) {
+  const int t = find_tensor(tab.first, tab.count, blockIdx.x);
+  const int64_t at = (int64_t)(blockIdx.x - tab.first[t]) * CHUNK;
+  T* p = (T*)tab.p[t] + at;
+  const T* g = (const T*)tab.g[t] + at;
+  uint8_t* m = (uint8_t*)tab.m[t] + at;
+  uint8_t* v = (uint8_t*)tab.v[t] + at;
+  const int b = threadIdx.x / 16, l = threadIdx.x % 16;
+  float2* scale = (float2*)tab.s[t] + at / QBLOCK + b;
+  const int64_t left = tab.n[t] - at;
+  const bool full = left >= CHUNK;
+  const float coef = clip_coef(norm, h.max_norm);
+  const int i0 = b * QBLOCK + l * 8;
+  const bool live = b * QBLOCK < left;  // the same for the 16 lanes
+  float pf[2][8], gf[2][8], mf[2][8], rf[2][8];
+  uint2 mc[2], vc[2];
+  const float2 s = live ? *scale : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = i0 + j * 128;
+    if (full) {
+      load_vec(g + i, gf[j]);
+      load_vec(p + i, pf[j]);
+      mc[j] = load_codes(m + i, 8);
+      vc[j] = load_codes(v + i, 8);
+    } else {
+      load_part(g + i, gf[j], left - i);
+      load_part(p + i, pf[j], left - i);
+      mc[j] = load_codes(m + i, left - i);
+      vc[j] = load_codes(v + i, left - i);
+    }
+  }
+  uint32_t top_m = __float_as_uint(TINY), top_r = __float_as_uint(TINY);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    decode8(mc[j], vc[j], mf[j], rf[j]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float r = rf[j][k] * s.y;
+      float v2 = r * r;
+      mf[j][k] *= s.x;
+      adamw_element(h, coef, gf[j][k], pf[j][k], mf[j][k], v2, rf[j][k]);
+      top_m = max(top_m, __float_as_uint(mf[j][k]) & 0x7FFFFFFFu);
+      top_r = max(top_r, __float_as_uint(rf[j][k]) & 0x7FFFFFFFu);
+    }
+  }
+  const float sm = __uint_as_float(max16(top_m)) * (float)(1.0 / 448.0);
+  const float sr = __uint_as_float(max16(top_r)) * (float)(1.0 / 1.9375);
+  const float im = __frcp_rn(sm), ir = __frcp_rn(sr);
+  const uint32_t key = seed + tab.key[t] + (uint32_t)at;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = i0 + j * 128;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      // clamped with comparisons: a NaN stays a NaN
+      const float q = mf[j][k] * im;
+      mf[j][k] = q > TOP_M ? TOP_M : q < -TOP_M ? -TOP_M : q;
+      w[k / 4] |= encode_root(rf[j][k] * ir, dither19(key + i + k))
+                  << (8 * (k % 4));
+    }
+    const uint2 mw = pack_m(mf[j]);
+    if (full) {
+      store_vec(p + i, pf[j]);
+      store_codes(m + i, mw, 8);
+      store_codes(v + i, make_uint2(w[0], w[1]), 8);
+    } else {
+      store_part(p + i, pf[j], left - i);
+      store_codes(m + i, mw, left - i);
+      store_codes(v + i, make_uint2(w[0], w[1]), left - i);
+    }
+  }
+  if (live && l == 0) *scale = make_float2(sm, sr);
+}
+
+// the moments of 8-bit codes, into p (m) and g (v) of the table
+template <typename T>
+__global__ __launch_bounds__(THREADS) void adamw8_values_kernel(
+    const AdamwTable tab) {
+  const int t = find_tensor(tab.first, tab.count, blockIdx.x);
+  const int64_t at = (int64_t)(blockIdx.x - tab.first[t]) * CHUNK;
+  const int64_t left = tab.n[t] - at;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = (j * THREADS + threadIdx.x) * 8;
+    const int64_t n = left - i;
+    if (n <= 0) break;
+    const uint2 mc = load_codes((const uint8_t*)tab.m[t] + at + i, n);
+    const uint2 vc = load_codes((const uint8_t*)tab.v[t] + at + i, n);
+    const float2 s = ((const float2*)tab.s[t])[(at + i) / QBLOCK];
+    float m[8], v[8];
+    decode8(mc, vc, m, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      m[k] *= s.x;
+      const float r = v[k] * s.y;
+      v[k] = r * r;
+    }
+    T* om = (T*)tab.p[t] + at + i;
+    T* ov = (T*)const_cast<void*>(tab.g[t]) + at + i;
+    if (n >= 8) {
+      store_vec(om, m);
+      store_vec(ov, v);
+    } else {
+      store_part(om, m, n);
+      store_part(ov, v, n);
+    }
+  }
+}
+
+// ---- gradient norm ---------------------------------------------------------
+// Squares and sums in 64 bits: a square of a 32-bit value is exact there,
+// and the order of the sum does not reach the 32-bit result.  Read-bound:
+// 4 (2) bytes an element.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void sumsq_kernel(
+    const AdamwTable tab, double* __restrict__ partial) {
+  constexpr int V = 16 / sizeof(T);
+  double acc = 0.0;
+  for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
+    const int t = find_tensor(tab.first, tab.count, c);
+    const int64_t at = (int64_t)(c - tab.first[t]) * CHUNK;
+    const T* g = (const T*)tab.g[t] + at;
+    const int64_t left = tab.n[t] - at;
+    float gf[V];
+    for (int i = threadIdx.x * V; i < CHUNK && i < left; i += THREADS * V) {
+      if (left - i >= V) load_vec(g + i, gf);
+      else load_part(g + i, gf, left - i);
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc += (double)gf[k] * (double)gf[k];
+    }
+  }
+  for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, WAVE);
+  __shared__ double part[THREADS / WAVE];
+  if (threadIdx.x % WAVE == 0) part[threadIdx.x / WAVE] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    partial[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__global__ __launch_bounds__(THREADS) void norm_final_kernel(
+    const double* __restrict__ partial, int n, float* __restrict__ out) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += THREADS) acc += partial[i];
+  for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, WAVE);
+  __shared__ double part[THREADS / WAVE];
+  if (threadIdx.x % WAVE == 0) part[threadIdx.x / WAVE] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *out = (float)sqrt((part[0] + part[1]) + (part[2] + part[3]));
+}
+
+template <typename T>
+void go_adamw(hipStream_t s, const AdamwTable& tab, const AdamwScalars& h,
+              const float* norm) {
+  adamw_kernel<T><<<dim3(tab.chunks), THREADS, 0, s>>>(tab, h, norm);
+}
+
+template <typename T>
+void go_adamw8(hipStream_t s, const AdamwTable& tab, const AdamwScalars& h,
+               const float* norm, uint32_t seed) {
+  adamw8_kernel<T><<<dim3(tab.chunks), THREADS, 0, s>>>(tab, h, norm, seed);
+}
+
+template <typename T>
+void go_values(hipStream_t s, const AdamwTable& tab) {
+  adamw8_values_kernel<T><<<dim3(tab.chunks), THREADS, 0, s>>>(tab);
+}
+
+template <typename T>
+void go_sumsq(hipStream_t s, const AdamwTable& tab, double* partial,
+              int blocks) {
+  sumsq_kernel<T><<<dim3(blocks), THREADS, 0, s>>>(tab, partial);
+}
+
+#define BY_DTYPE(dtype, fn, ...)                        \
+  switch (dtype) {                                      \
+    case 0: fn<float>(__VA_ARGS__); break;              \
+    case 1: fn<__bf16>(__VA_ARGS__); break;             \
+    case 2: fn<_Float16>(__VA_ARGS__); break;           \
+    default: return (int)hipErrorInvalidValue;          \
+  }
+
+}  // namespace
+
+extern "C" int launch_adamw(void* stream, const AdamwTable* tab,
+                            const AdamwScalars* h, const float* norm,
+                            int dtype) {
+  if (tab->chunks == 0) return 0;
+  BY_DTYPE(dtype, go_adamw, (hipStream_t)stream, *tab, *h, norm)
+  HIP_CHECK_LAST();
+  return 0;
+}
+
+extern "C" int launch_adamw8(void* stream, const AdamwTable* tab,
+                             const AdamwScalars* h, const float* norm,
+                             int dtype, uint32_t seed) {
+  if (tab->chunks == 0) return 0;
+  BY_DTYPE(dtype, go_adamw8, (hipStream_t)stream, *tab, *h, norm, seed)
+  HIP_CHECK_LAST();
+  return 0;
+}
+
+extern "C" int launch_adamw8_values(void* stream, const AdamwTable* tab,
+                                    int dtype) {
+  if (tab->chunks == 0) return 0;
+  BY_DTYPE(dtype, go_values, (hipStream_t)stream, *tab)
+  HIP_CHECK_LAST();
+  return 0;
+}
+
+extern "C" int launch_sumsq(void* stream, const AdamwTable* tab, int dtype,
+                            double* partial, int blocks) {
+  if (tab->chunks == 0 || blocks == 0) return 0;
+  BY_DTYPE(dtype, go_sumsq, (hipStream_t)stream, *tab, partial, blocks)
+  HIP_CHECK_LAST();
+  return 0;
+}
+
+extern "C" int launch_norm_final(void* stream, const double* partial, int n,
+                                 float* out) {
+  norm_final_kernel<<<dim3(1), THREADS, 0, (hipStream_t)stream>>>(partial, n,
+                                                                  out);
+  HIP_CHECK_LAST();
+  return 0;
+}

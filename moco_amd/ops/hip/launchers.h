@@ -56,6 +56,44 @@ int launch_multi_tensor_sgd(void* stream, const int64_t* ptrs_p,
 int launch_ema_flat(void* stream, float* dst, const float* src, int64_t n,
                     float m);
 
+// ---- adamw.hip ------------------------------------------------------------
+// A table of up to ADAMW_TENSORS tensors of one dtype, passed by value in
+// the kernel's arguments.  Tensor i has n[i] elements, at p (weights), g
+// (gradients), m and v (moments, fp32 or 8-bit codes) and s (fp32 pairs of
+// scales, one per 256 elements; 8-bit only), and takes the chunks of
+// ADAMW_CHUNK elements from first[i] on; key[i] is its number in the
+// caller's list, spread over 32 bits.  dtype: 0 fp32, 1 bf16, 2 fp16.
+#define ADAMW_TENSORS 64
+#define ADAMW_CHUNK 4096
+struct AdamwTable {
+  void* p[ADAMW_TENSORS];
+  const void* g[ADAMW_TENSORS];
+  void* m[ADAMW_TENSORS];
+  void* v[ADAMW_TENSORS];
+  void* s[ADAMW_TENSORS];
+  int64_t n[ADAMW_TENSORS];
+  uint32_t first[ADAMW_TENSORS];
+  uint32_t key[ADAMW_TENSORS];
+  uint32_t chunks;
+  int count;
+};
+struct AdamwScalars {
+  float beta1, one_minus_beta1, beta2, one_minus_beta2;
+  float inv_root_bc2, eps, decay, step_size, max_norm;
+};
+// norm: device fp32 scalar for the clip, or null for none
+int launch_adamw(void* stream, const AdamwTable* tab, const AdamwScalars* h,
+                 const float* norm, int dtype);
+int launch_adamw8(void* stream, const AdamwTable* tab, const AdamwScalars* h,
+                  const float* norm, int dtype, uint32_t seed);
+// decoded moments of the codes m, v, s into p (m) and g (v), of type dtype
+int launch_adamw8_values(void* stream, const AdamwTable* tab, int dtype);
+// partial[blocks]: sums of squares of the table's g
+int launch_sumsq(void* stream, const AdamwTable* tab, int dtype,
+                 double* partial, int blocks);
+// out = sqrt(sum of partial[0..n))
+int launch_norm_final(void* stream, const double* partial, int n, float* out);
+
 // ---- bn.hip ---------------------------------------------------------------
 // x/y/g/res: [R, C] bf16 (NHWC flattened); stats fp32; C in {64..256 dividing
 // 256, or multiples of 256 up to 2048}; part_* workspaces are [304, C] fp32.
