@@ -78,6 +78,7 @@ from .adamw import (  # noqa: E402
     adamw_,
     grad_norm,
 )
+from .norm_residual import norm_residual  # noqa: E402
 from .augment import two_crop_augment  # noqa: E402
 
 __all__ = [
@@ -96,5 +97,6 @@ __all__ = [
     "adamw8bit_",
     "adamw8bit_values",
     "grad_norm",
+    "norm_residual",
     "two_crop_augment",
 ]

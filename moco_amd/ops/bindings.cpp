@@ -302,11 +302,11 @@ struct TableFiller {
   void add(void* p, const void* g, void* m, void* v, void* s, int64_t n,
            uint32_t key) {
     const int64_t chunks = (n + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
-    TORCH_CHECK_VALUE(chunks < (int64_t)1 << 30, "a tensor of ", n,
+    // a grid holds fewer than 2^32 threads, 256 of them a chunk
+    constexpr int64_t MOST = ((int64_t)1 << 24) - 1;
+    TORCH_CHECK_VALUE(chunks <= MOST, "a tensor of ", n,
                       " elements is too large");
-    if (tab.count == ADAMW_TENSORS ||
-        (int64_t)tab.chunks + chunks > (int64_t)1 << 30)
-      flush();
+    if (tab.count == ADAMW_TENSORS || tab.chunks + chunks > MOST) flush();
     const int i = tab.count++;
     tab.p[i] = p, tab.g[i] = g, tab.m[i] = m, tab.v[i] = v, tab.s[i] = s;
     tab.n[i] = n, tab.first[i] = tab.chunks, tab.key[i] = key;
@@ -507,6 +507,211 @@ std::vector<TensorList> adamw8bit_values(const TensorList& ms,
     out[1].push_back(ov);
   }
   fill.flush();
+  return out;
+}
+
+// ---------------------------------------------------------------------------
+// Norms after and before a residual block (norm_residual.hip)
+
+using OptTensor = c10::optional<torch::Tensor>;
+
+// A tensor whose rows (all but the last dimension) lie at equal distances,
+// each without gaps: the tensor itself, or a contiguous copy of it.
+struct Rows {
+  torch::Tensor t;
+  int64_t ld = 0;
+  Rows() = default;
+  explicit Rows(const torch::Tensor& in) : t(in) {
+    const int64_t width = in.size(-1);
+    ld = width;
+    bool ok = width <= 1 || in.stride(-1) == 1;
+    int64_t want = -1;  // stride that the next dimension outwards must have
+    for (int64_t d = in.dim() - 2; ok && d >= 0; --d) {
+      if (in.size(d) == 1) continue;
+      if (want < 0) ld = in.stride(d);
+      else ok = in.stride(d) == want;
+      want = in.stride(d) * in.size(d);
+    }
+    if (!ok) {
+      t = in.contiguous();
+      ld = width;
+    }
+  }
+};
+
+struct NormCall {
+  NormArgs a{};
+  Rows x, h, gate;
+  std::vector<torch::Tensor> keep;  // vectors, made contiguous
+
+  const void* vec(const OptTensor& v, int bit) {
+    if (!v.has_value()) return nullptr;
+    TORCH_CHECK_VALUE(v->is_cuda() && v->device() == x.t.device() &&
+                          v->dim() == 1 && v->size(0) == a.width,
+                      "a weight, bias or scale must be [", a.width,
+                      "] on the device of x");
+    const int type = adamw_dtype(*v, "weights, biases and scale");
+    TORCH_CHECK_TYPE(type == 0 || type == a.type_h, "weights, biases and "
+                     "scale must be float32 or of the block's type, got ",
+                     v->scalar_type());
+    if (type == 0) a.f32 |= 1 << bit;
+    keep.push_back(v->contiguous());
+    return keep.back().const_data_ptr();
+  }
+
+  NormCall(const torch::Tensor& x_in, const OptTensor& h_in,
+           const OptTensor& gate_in, const OptTensor& w1, const OptTensor& b1,
+           const OptTensor& w2, const OptTensor& b2, const OptTensor& scale,
+           double scale_value, int64_t post, int64_t pre, int64_t act,
+           double post_eps, double pre_eps, int type_y) {
+    TORCH_CHECK_VALUE(x_in.is_cuda() && x_in.dim() >= 1 && x_in.size(-1) > 0,
+                      "x must be a GPU tensor [..., width]");
+    TORCH_CHECK_VALUE(x_in.size(-1) <= NORM_MAX_WIDTH, "a width of ",
+                      x_in.size(-1), " is over ", NORM_MAX_WIDTH);
+    x = Rows(x_in);
+    a.width = (int)x_in.size(-1);
+    a.rows = x_in.numel() / a.width;
+    a.type_x = adamw_dtype(x_in, "x");
+    a.type_h = type_y;
+    a.x = x.t.const_data_ptr(), a.ld_x = x.ld;
+    if (h_in.has_value()) {
+      TORCH_CHECK_VALUE(h_in->sizes() == x_in.sizes() &&
+                            h_in->device() == x_in.device(),
+                        "branch must have x's shape and device");
+      a.type_h = adamw_dtype(*h_in, "branch");
+      h = Rows(*h_in);
+      a.h = h.t.const_data_ptr(), a.ld_h = h.ld;
+    }
+    TORCH_CHECK_TYPE(a.type_x == 0 || a.type_x == a.type_h,
+                     "x must be float32 or of the block's type");
+    if (gate_in.has_value()) {
+      const auto& g = *gate_in;
+      TORCH_CHECK_VALUE(h_in.has_value() && g.device() == x_in.device() &&
+                            g.dim() == x_in.dim() &&
+                            g.sizes().slice(0, g.dim() - 1) ==
+                                x_in.sizes().slice(0, x_in.dim() - 1) &&
+                            (g.size(-1) == a.width || g.size(-1) == 1),
+                        "gate must have the branch's shape, or 1 as its last "
+                        "dimension");
+      TORCH_CHECK_TYPE(adamw_dtype(g, "gate") == a.type_h,
+                       "gate must be of the branch's type");
+      a.gate_kind = g.size(-1) == a.width ? NORM_GATE_FULL : NORM_GATE_ROW;
+      gate = Rows(g);
+      a.gate = gate.t.const_data_ptr(), a.ld_g = gate.ld;
+    }
+    TORCH_CHECK_VALUE(post >= 0 && post <= 2 && pre >= 0 && pre <= 2 &&
+                      act >= 0 && act <= 2, "unknown norm or gate");
+    a.post = (int)post, a.pre = (int)pre, a.act = (int)act;
+    a.scale_value = (float)scale_value;
+    a.post_eps = (float)post_eps, a.pre_eps = (float)pre_eps;
+    a.w1 = vec(w1, 0), a.b1 = vec(b1, 1), a.w2 = vec(w2, 2);
+    a.b2 = vec(b2, 3), a.scale = vec(scale, 4);
+  }
+};
+
+torch::ScalarType norm_type(int t) {
+  return t == 0 ? torch::kFloat32 : t == 1 ? torch::kBFloat16 : torch::kHalf;
+}
+
+// {r, y, stats}; undefined where there is none
+std::vector<OptTensor> norm_residual_fwd(
+    const torch::Tensor& x, const OptTensor& h, const OptTensor& gate,
+    const OptTensor& w1, const OptTensor& b1, const OptTensor& w2,
+    const OptTensor& b2, const OptTensor& scale, double scale_value,
+    int64_t post, int64_t pre, int64_t act, double post_eps, double pre_eps,
+    int64_t type_y, bool want_stats) {
+  at::cuda::OptionalCUDAGuard guard(x.device());
+  NormCall c(x, h, gate, w1, b1, w2, b2, scale, scale_value, post, pre, act,
+             post_eps, pre_eps, (int)type_y);
+  std::vector<OptTensor> out(3);
+  auto opts = x.options();
+  if (h.has_value()) {
+    out[0] = torch::empty(x.sizes(), opts);
+    c.a.r = out[0]->data_ptr();
+  }
+  if (pre != NORM_NONE) {
+    out[1] = torch::empty(x.sizes(), opts.dtype(norm_type(c.a.type_h)));
+    c.a.y = out[1]->data_ptr();
+  }
+  if (want_stats) {
+    out[2] = torch::empty({4, c.a.rows}, opts.dtype(torch::kFloat32));
+    c.a.stats = out[2]->data_ptr<float>();
+  }
+  CHECK_LAUNCH(launch_norm_fwd(cur_stream(), &c.a));
+  return out;
+}
+
+// {dx, dh, dgate, dw1, db1, dw2, db2, dscale}, those that `want` has a bit
+// for
+std::vector<OptTensor> norm_residual_bwd(
+    const OptTensor& d_r, const OptTensor& d_y, const torch::Tensor& stats,
+    const torch::Tensor& x, const OptTensor& h, const OptTensor& gate,
+    const OptTensor& w1, const OptTensor& b1, const OptTensor& w2,
+    const OptTensor& b2, const OptTensor& scale, double scale_value,
+    int64_t post, int64_t pre, int64_t act, double post_eps, double pre_eps,
+    int64_t type_y, int64_t want) {
+  at::cuda::OptionalCUDAGuard guard(x.device());
+  NormCall c(x, h, gate, w1, b1, w2, b2, scale, scale_value, post, pre, act,
+             post_eps, pre_eps, (int)type_y);
+  TORCH_CHECK(stats.is_cuda() && stats.is_contiguous() &&
+              stats.scalar_type() == torch::kFloat32 &&
+              stats.numel() == 4 * c.a.rows);
+  c.a.stats = stats.data_ptr<float>();
+  NormGrads o{};
+  auto opts = x.options();
+  const auto type_h = norm_type(c.a.type_h);
+  torch::Tensor dr, dy;
+  if (d_r.has_value()) {
+    TORCH_CHECK(d_r->sizes() == x.sizes() &&
+                d_r->scalar_type() == x.scalar_type() &&
+                d_r->device() == x.device());
+    dr = d_r->contiguous();
+    o.d_r = dr.const_data_ptr();
+  }
+  if (d_y.has_value()) {
+    TORCH_CHECK(d_y->sizes() == x.sizes() && d_y->scalar_type() == type_h &&
+                d_y->device() == x.device() && pre != NORM_NONE);
+    dy = d_y->contiguous();
+    o.d_y = dy.const_data_ptr();
+  }
+  std::vector<OptTensor> out(8);
+  if (want & 1) {
+    out[0] = torch::empty(x.sizes(), opts);
+    o.d_x = out[0]->data_ptr();
+  }
+  if ((want & 2) && h.has_value()) {
+    out[1] = torch::empty(x.sizes(), opts.dtype(type_h));
+    o.d_h = out[1]->data_ptr();
+  }
+  if ((want & 4) && gate.has_value()) {
+    out[2] = torch::empty(gate->sizes(), opts.dtype(type_h));
+    o.d_gate = out[2]->data_ptr();
+  }
+  const OptTensor* vec[5] = {&w1, &b1, &w2, &b2, &scale};
+  const int blocks = norm_bwd_blocks(c.a.rows, c.a.width);
+  const int64_t slab = (int64_t)blocks * c.a.width;
+  int vecs = 0;
+  for (int j = 0; j < 5; ++j)
+    vecs += ((want >> (3 + j)) & 1) && vec[j]->has_value();
+  auto partial = torch::empty({vecs * slab}, opts.dtype(torch::kFloat32));
+  NormColumns cols{};
+  int used = 0;
+  for (int j = 0; j < 5; ++j) {
+    if (!((want >> (3 + j)) & 1) || !vec[j]->has_value()) continue;
+    auto& d = out[3 + j];
+    // no rows: nothing is launched, and the sums are zero
+    d = c.a.rows ? torch::empty_like(**vec[j], at::MemoryFormat::Contiguous)
+                 : torch::zeros_like(**vec[j], at::MemoryFormat::Contiguous);
+    o.partial[j] = partial.data_ptr<float>() + used * slab;
+    cols.partial[used] = o.partial[j];
+    cols.out[used] = d->data_ptr();
+    cols.dtype[used++] = adamw_dtype(*d, "weights, biases and scale");
+  }
+  if (c.a.rows) {
+    CHECK_LAUNCH(launch_norm_bwd(cur_stream(), &c.a, &o, blocks));
+    CHECK_LAUNCH(launch_norm_columns(cur_stream(), &cols, vecs, blocks,
+                                     c.a.width));
+  }
   return out;
 }
 
@@ -986,6 +1191,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("multi_tensor_sgd", &multi_tensor_sgd);
   mod.def("ema_flat", &ema_flat);
   mod.def("grad_norm", &grad_norm);
+  mod.def("norm_residual_fwd", &norm_residual_fwd);
+  mod.def("norm_residual_bwd", &norm_residual_bwd);
   mod.def("adamw_step", &adamw_step);
   mod.def("adamw8bit_values", [](const TensorList& m, const TensorList& v,
                                  const TensorList& s, py::object dtype) {

@@ -94,6 +94,45 @@ int launch_sumsq(void* stream, const AdamwTable* tab, int dtype,
 // out = sqrt(sum of partial[0..n))
 int launch_norm_final(void* stream, const double* partial, int n, float* out);
 
+// ---- norm_residual.hip ----------------------------------------------------
+// x, r: [rows, width] of type_x; h, gate, y: of type_h (0 fp32, 1 bf16,
+// 2 fp16; type_x is fp32 or type_h).  ld_*: elements from row to row of the
+// inputs; outputs are contiguous.  w1, b1, scale, w2, b2: [width], null for
+// none; bit j of f32: the j-th of (w1, b1, w2, b2, scale) is fp32, else
+// type_h.  stats: fp32 [4, rows] (mean and 1/std after, then before), null
+// where no backward follows.
+enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
+enum { NORM_GATE_NONE = 0, NORM_GATE_FULL = 1, NORM_GATE_ROW = 2 };
+enum { NORM_ACT_NONE = 0, NORM_ACT_SIGMOID = 1, NORM_ACT_SILU = 2 };
+#define NORM_MAX_WIDTH 16384
+struct NormArgs {
+  const void *x, *h, *gate, *w1, *b1, *w2, *b2, *scale;
+  void *r, *y;
+  float* stats;
+  int64_t rows, ld_x, ld_h, ld_g;
+  int width, type_x, type_h, post, pre, gate_kind, act, f32;
+  float scale_value, post_eps, pre_eps;
+};
+// d_r, d_y: contiguous, null where an output has no gradient; d_x, d_h,
+// d_gate: null where none is wanted; partial[j]: fp32 [blocks, width] for
+// the column sums of dw1, db1, dw2, db2, dscale, null where none is wanted
+struct NormGrads {
+  const void *d_r, *d_y;
+  void *d_x, *d_h, *d_gate;
+  float* partial[5];
+};
+struct NormColumns {
+  const float* partial[5];
+  void* out[5];
+  int dtype[5];
+};
+int launch_norm_fwd(void* stream, const NormArgs* a);
+int norm_bwd_blocks(int64_t rows, int64_t width);
+int launch_norm_bwd(void* stream, const NormArgs* a, const NormGrads* o,
+                    int blocks);
+int launch_norm_columns(void* stream, const NormColumns* v, int vecs,
+                        int blocks, int64_t width);
+
 // ---- bn.hip ---------------------------------------------------------------
 // x/y/g/res: [R, C] bf16 (NHWC flattened); stats fp32; C in {64..256 dividing
 // 256, or multiples of 256 up to 2048}; part_* workspaces are [304, C] fp32.

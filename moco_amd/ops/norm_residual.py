@@ -1,0 +1,191 @@
+"""The norms after and before a residual block, with its gate and residual
+scale, as one op: where one block ends and the next begins.
+
+Beside bn_act (bn.py), which does the same for convolution blocks: there the
+norm is over the batch, here over the last dimension (RMSNorm, LayerNorm).
+GPU path: ops/hip/norm_residual.hip.  The reference has batch norms only.
+"""
+
+from typing import Optional, Tuple, Union
+
+import torch
+import torch.nn as nn
+
+from . import ext, use_hip
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTS = {None: 0, "sigmoid": 1, "silu": 2}
+
+Norm = Union[nn.RMSNorm, nn.LayerNorm]
+
+
+def _norm_args(mod: Optional[Norm], width: int, which: str):
+    """(kind, weight, bias, eps) of a norm module."""
+    if mod is None:
+        return 0, None, None, 0.0
+    if isinstance(mod, nn.RMSNorm):
+        kind, bias = 1, None
+    elif isinstance(mod, nn.LayerNorm):
+        kind, bias = 2, mod.bias
+    else:
+        raise TypeError(f"{which} must be an nn.RMSNorm or nn.LayerNorm, got "
+                        f"{type(mod).__name__}")
+    if tuple(mod.normalized_shape) != (width,):
+        raise ValueError(f"{which} normalizes {tuple(mod.normalized_shape)}, "
+                         f"the last dimension is {width}")
+    if mod.eps is None or not mod.eps >= 0.0:
+        raise ValueError(f"{which} needs an eps of its own, got {mod.eps}")
+    return kind, mod.weight, bias, mod.eps
+
+
+class _NormResidual(torch.autograd.Function):
+    """Tensors: x, branch, gate, post weight and bias, pre weight and bias,
+    scale."""
+
+    @staticmethod
+    def forward(ctx, numbers, *tensors):
+        r, y, stats = ext().norm_residual_fwd(*tensors, *numbers, True)
+        ctx.save_for_backward(stats, *tensors)
+        ctx.numbers = numbers
+        ctx.set_materialize_grads(False)
+        return r, y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_r, d_y):
+        if d_r is None and d_y is None:
+            return (None,) * 9
+        want = sum(1 << i for i, w in enumerate(ctx.needs_input_grad[1:])
+                   if w)
+        stats, *tensors = ctx.saved_tensors
+        return (None, *ext().norm_residual_bwd(d_r, d_y, stats, *tensors,
+                                               *ctx.numbers, want))
+
+
+def _plain_norm(x, kind, weight, bias, eps):
+    if kind == 0:
+        return x
+    if kind == 2:
+        x = x - x.mean(-1, keepdim=True)
+    y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight.to(y.dtype)
+    return y if bias is None else y + bias.to(y.dtype)
+
+
+def _plain(x, branch, gate, w1, b1, w2, b2, scale, scale_value, post, pre,
+           act, eps1, eps2, out_dtype):
+    """The same in elementary operations, in 32 bits (64 for float64)."""
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    r = x.to(wide)
+    if branch is not None:
+        add = _plain_norm(branch.to(wide), post, w1, b1, eps1)
+        if gate is not None:
+            g = gate.to(wide)
+            s = torch.sigmoid(g)
+            add = add * (g if act == 0 else s if act == 1 else g * s)
+        r = r + add * (scale_value if scale is None else scale.to(wide))
+    y = _plain_norm(r, pre, w2, b2, eps2).to(out_dtype) if pre else None
+    return r.to(x.dtype), y
+
+
+def norm_residual(x: torch.Tensor, branch: Optional[torch.Tensor] = None, *,
+                  post: Optional[Norm] = None, pre: Optional[Norm] = None,
+                  gate: Optional[torch.Tensor] = None,
+                  gate_act: Optional[str] = None,
+                  scale: Union[None, float, torch.Tensor] = None,
+                  out_dtype: Optional[torch.dtype] = None
+                  ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``r = x + scale * act(gate) * post(branch);  y = pre(r)``.
+
+    Ends one residual block and begins the next: `branch` is what a block put
+    out, `post` the norm after it (sandwich norms), `pre` the norm before the
+    next block.  Returns (r, y): the residual stream and the next block's
+    input; y is None without `pre`.  Without `branch` (the first block) r is
+    x and only y is computed.
+
+    x: [..., width], the residual stream; float32, or of the branch's type.
+    branch: x's shape; float32, bfloat16 or float16, and the type of y.
+    post, pre: nn.RMSNorm or nn.LayerNorm over the last dimension, with or
+        without weight and bias; None for no norm.
+    gate: the branch's shape, or [..., 1] for one gate per token, of the
+        branch's type; gate_act: None, "sigmoid" or "silu".
+    scale: a number, or a tensor [width] (or of one element).  Weights,
+        biases and scale are float32 or of the branch's type.
+    out_dtype: type of y where there is no branch (x's by default).
+
+    Everything is computed in 32 bits from the inputs: y is the norm of r
+    before r is rounded to x's type.  Gradients flow to every tensor; x,
+    branch and gate may be strided (halves of one projection) as long as the
+    last dimension is dense, other layouts are copied.  On the GPU width is
+    16384 at most.
+    """
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [..., width], got {tuple(x.shape)}")
+    width = x.shape[-1]
+    post_kind, w1, b1, eps1 = _norm_args(post, width, "post")
+    pre_kind, w2, b2, eps2 = _norm_args(pre, width, "pre")
+    if gate_act not in _ACTS:
+        raise ValueError(f"gate_act must be None, 'sigmoid' or 'silu', got "
+                         f"{gate_act!r}")
+    if branch is None:
+        if post is not None or gate is not None or scale is not None:
+            raise ValueError("post, gate and scale need a branch")
+        if pre is None:
+            raise ValueError("neither a branch nor a norm is given")
+        block_type = out_dtype or x.dtype
+    else:
+        block_type = branch.dtype
+        if out_dtype not in (None, block_type):
+            raise ValueError("y has the branch's type: out_dtype is for calls "
+                             "without one")
+        if branch.shape != x.shape:
+            raise ValueError(f"branch is {tuple(branch.shape)}, x "
+                             f"{tuple(x.shape)}")
+    if gate is None:
+        if gate_act is not None:
+            raise ValueError("gate_act needs a gate")
+    elif gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or \
+            gate.shape[-1] not in (1, width):
+        raise ValueError(f"gate must be {tuple(x.shape)} or have 1 as its "
+                         f"last dimension, got {tuple(gate.shape)}")
+    scale_value = 1.0
+    if isinstance(scale, torch.Tensor):
+        if scale.numel() == 1 and width > 1:
+            scale = scale.reshape(1).expand(width)
+        if scale.shape != (width,):
+            raise ValueError(f"scale must be a number or [{width}], got "
+                             f"{tuple(scale.shape)}")
+    elif scale is not None:
+        scale, scale_value = None, float(scale)
+    if x.dtype not in (torch.float32, block_type):
+        raise TypeError(f"x must be float32 or of the block's type, got "
+                        f"{x.dtype} with {block_type}")
+    if gate is not None and gate.dtype != block_type:
+        raise TypeError(f"gate is {gate.dtype}, the branch {block_type}")
+    tensors = (x, branch, gate, w1, b1, w2, b2, scale)
+    for t in tensors[3:]:
+        if t is not None and t.dtype not in (torch.float32, block_type):
+            raise TypeError("weights, biases and scale must be float32 or of "
+                            f"the block's type, got {t.dtype}")
+    if any(t is not None and t.device != x.device for t in tensors):
+        raise ValueError("all tensors must be on one device")
+
+    if use_hip(x):
+        if block_type not in _TYPES:
+            raise TypeError(f"on the GPU the block's type is float32, "
+                            f"bfloat16 or float16, got {block_type}")
+        numbers = (scale_value, post_kind, pre_kind, _ACTS[gate_act], eps1,
+                   eps2, _TYPES[block_type])
+        if torch.is_grad_enabled() and any(
+                t is not None and t.requires_grad for t in tensors):
+            r, y = _NormResidual.apply(numbers, *tensors)
+        else:
+            r, y, _ = ext().norm_residual_fwd(*tensors, *numbers, False)
+    else:
+        if block_type not in _TYPES and block_type != torch.float64:
+            raise TypeError(f"the block's type must be a float type, got "
+                            f"{block_type}")
+        r, y = _plain(*tensors, scale_value, post_kind, pre_kind,
+                      _ACTS[gate_act], eps1, eps2, block_type)
+    return (x if branch is None else r), y

@@ -23,6 +23,7 @@ sources = [
     "moco_amd/ops/hip/softmax_ce.hip",
     "moco_amd/ops/hip/multi_tensor.hip",
     "moco_amd/ops/hip/adamw.hip",
+    "moco_amd/ops/hip/norm_residual.hip",
     "moco_amd/ops/hip/queue.hip",
     "moco_amd/ops/hip/bn.hip",
     "moco_amd/ops/hip/pool.hip",
