@@ -6,7 +6,11 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <algorithm>
+#include <array>
 #include <cmath>
 
 #include "hip/launchers.h"
@@ -613,29 +617,35 @@ torch::ScalarType norm_type(int t) {
   return t == 0 ? torch::kFloat32 : t == 1 ? torch::kBFloat16 : torch::kHalf;
 }
 
+// what is not a tensor of a call
+struct NormNumbers {
+  double scale_value, post_eps, pre_eps;
+  int64_t post, pre, act, type_y;
+};
+
 // {r, y, stats}; undefined where there is none
-std::vector<OptTensor> norm_residual_fwd(
+std::array<torch::Tensor, 3> norm_residual_fwd(
     const torch::Tensor& x, const OptTensor& h, const OptTensor& gate,
     const OptTensor& w1, const OptTensor& b1, const OptTensor& w2,
-    const OptTensor& b2, const OptTensor& scale, double scale_value,
-    int64_t post, int64_t pre, int64_t act, double post_eps, double pre_eps,
-    int64_t type_y, bool want_stats) {
-  at::cuda::OptionalCUDAGuard guard(x.device());
-  NormCall c(x, h, gate, w1, b1, w2, b2, scale, scale_value, post, pre, act,
-             post_eps, pre_eps, (int)type_y);
-  std::vector<OptTensor> out(3);
-  auto opts = x.options();
+    const OptTensor& b2, const OptTensor& scale, const NormNumbers& num,
+    bool want_stats) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a GPU tensor");
+  at::cuda::CUDAGuard guard(x.device());
+  NormCall c(x, h, gate, w1, b1, w2, b2, scale, num.scale_value, num.post,
+             num.pre, num.act, num.post_eps, num.pre_eps, (int)num.type_y);
+  std::array<torch::Tensor, 3> out;
+  auto opts = x.options().requires_grad(false);
   if (h.has_value()) {
     out[0] = torch::empty(x.sizes(), opts);
-    c.a.r = out[0]->data_ptr();
+    c.a.r = out[0].data_ptr();
   }
-  if (pre != NORM_NONE) {
+  if (num.pre != NORM_NONE) {
     out[1] = torch::empty(x.sizes(), opts.dtype(norm_type(c.a.type_h)));
-    c.a.y = out[1]->data_ptr();
+    c.a.y = out[1].data_ptr();
   }
   if (want_stats) {
     out[2] = torch::empty({4, c.a.rows}, opts.dtype(torch::kFloat32));
-    c.a.stats = out[2]->data_ptr<float>();
+    c.a.stats = out[2].data_ptr<float>();
   }
   CHECK_LAUNCH(launch_norm_fwd(cur_stream(), &c.a));
   return out;
@@ -643,22 +653,21 @@ std::vector<OptTensor> norm_residual_fwd(
 
 // {dx, dh, dgate, dw1, db1, dw2, db2, dscale}, those that `want` has a bit
 // for
-std::vector<OptTensor> norm_residual_bwd(
+std::vector<torch::Tensor> norm_residual_bwd(
     const OptTensor& d_r, const OptTensor& d_y, const torch::Tensor& stats,
     const torch::Tensor& x, const OptTensor& h, const OptTensor& gate,
     const OptTensor& w1, const OptTensor& b1, const OptTensor& w2,
-    const OptTensor& b2, const OptTensor& scale, double scale_value,
-    int64_t post, int64_t pre, int64_t act, double post_eps, double pre_eps,
-    int64_t type_y, int64_t want) {
-  at::cuda::OptionalCUDAGuard guard(x.device());
-  NormCall c(x, h, gate, w1, b1, w2, b2, scale, scale_value, post, pre, act,
-             post_eps, pre_eps, (int)type_y);
+    const OptTensor& b2, const OptTensor& scale, const NormNumbers& num,
+    int64_t want) {
+  at::cuda::CUDAGuard guard(x.device());
+  NormCall c(x, h, gate, w1, b1, w2, b2, scale, num.scale_value, num.post,
+             num.pre, num.act, num.post_eps, num.pre_eps, (int)num.type_y);
   TORCH_CHECK(stats.is_cuda() && stats.is_contiguous() &&
               stats.scalar_type() == torch::kFloat32 &&
               stats.numel() == 4 * c.a.rows);
   c.a.stats = stats.data_ptr<float>();
   NormGrads o{};
-  auto opts = x.options();
+  auto opts = x.options().requires_grad(false);
   const auto type_h = norm_type(c.a.type_h);
   torch::Tensor dr, dy;
   if (d_r.has_value()) {
@@ -670,22 +679,22 @@ std::vector<OptTensor> norm_residual_bwd(
   }
   if (d_y.has_value()) {
     TORCH_CHECK(d_y->sizes() == x.sizes() && d_y->scalar_type() == type_h &&
-                d_y->device() == x.device() && pre != NORM_NONE);
+                d_y->device() == x.device() && num.pre != NORM_NONE);
     dy = d_y->contiguous();
     o.d_y = dy.const_data_ptr();
   }
-  std::vector<OptTensor> out(8);
+  std::vector<torch::Tensor> out(8);
   if (want & 1) {
     out[0] = torch::empty(x.sizes(), opts);
-    o.d_x = out[0]->data_ptr();
+    o.d_x = out[0].data_ptr();
   }
   if ((want & 2) && h.has_value()) {
     out[1] = torch::empty(x.sizes(), opts.dtype(type_h));
-    o.d_h = out[1]->data_ptr();
+    o.d_h = out[1].data_ptr();
   }
   if ((want & 4) && gate.has_value()) {
     out[2] = torch::empty(gate->sizes(), opts.dtype(type_h));
-    o.d_gate = out[2]->data_ptr();
+    o.d_gate = out[2].data_ptr();
   }
   const OptTensor* vec[5] = {&w1, &b1, &w2, &b2, &scale};
   const int blocks = norm_bwd_blocks(c.a.rows, c.a.width);
@@ -700,17 +709,113 @@ std::vector<OptTensor> norm_residual_bwd(
     if (!((want >> (3 + j)) & 1) || !vec[j]->has_value()) continue;
     auto& d = out[3 + j];
     // no rows: nothing is launched, and the sums are zero
-    d = c.a.rows ? torch::empty_like(**vec[j], at::MemoryFormat::Contiguous)
-                 : torch::zeros_like(**vec[j], at::MemoryFormat::Contiguous);
+    const auto vo = (*vec[j])->options().requires_grad(false);
+    d = c.a.rows ? torch::empty({c.a.width}, vo)
+                 : torch::zeros({c.a.width}, vo);
     o.partial[j] = partial.data_ptr<float>() + used * slab;
     cols.partial[used] = o.partial[j];
-    cols.out[used] = d->data_ptr();
-    cols.dtype[used++] = adamw_dtype(*d, "weights, biases and scale");
+    cols.out[used] = d.data_ptr();
+    cols.dtype[used++] = adamw_dtype(d, "weights, biases and scale");
   }
   if (c.a.rows) {
     CHECK_LAUNCH(launch_norm_bwd(cur_stream(), &c.a, &o, blocks));
     CHECK_LAUNCH(launch_norm_columns(cur_stream(), &cols, vecs, blocks,
                                      c.a.width));
+  }
+  return out;
+}
+
+class NormResidual : public torch::autograd::Function<NormResidual> {
+ public:
+  // {r, y}, those that there are
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext* ctx, const torch::Tensor& x,
+      const OptTensor& h, const OptTensor& gate, const OptTensor& w1,
+      const OptTensor& b1, const OptTensor& w2, const OptTensor& b2,
+      const OptTensor& scale, double scale_value, int64_t post, int64_t pre,
+      int64_t act, double post_eps, double pre_eps, int64_t type_y) {
+    const NormNumbers num{scale_value, post_eps, pre_eps, post,
+                          pre,         act,      type_y};
+    auto out = norm_residual_fwd(x, h, gate, w1, b1, w2, b2, scale, num, true);
+    const OptTensor* rest[7] = {&h, &gate, &w1, &b1, &w2, &b2, &scale};
+    torch::autograd::variable_list keep{x};
+    for (auto* t : rest) keep.push_back(t->value_or(torch::Tensor()));
+    keep.push_back(out[2]);
+    ctx->save_for_backward(keep);
+    ctx->saved_data["numbers"] =
+        std::vector<double>{scale_value,  post_eps,    pre_eps,
+                            (double)post, (double)pre, (double)act,
+                            (double)type_y};
+    ctx->set_materialize_grads(false);
+    torch::autograd::variable_list result;
+    for (int i = 0; i < 2; ++i)
+      if (out[i].defined()) result.push_back(out[i]);
+    return result;
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    torch::autograd::variable_list result(15);
+    const auto saved = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["numbers"].toDoubleVector();
+    const NormNumbers num{n[0],          n[1],          n[2],
+                          (int64_t)n[3], (int64_t)n[4], (int64_t)n[5],
+                          (int64_t)n[6]};
+    auto opt = [](const torch::Tensor& t) {
+      return t.defined() ? OptTensor(t) : OptTensor();
+    };
+    size_t at = 0;
+    OptTensor d_r, d_y;
+    if (saved[1].defined()) d_r = opt(grads.at(at++));
+    if (num.pre != NORM_NONE) d_y = opt(grads.at(at++));
+    if (!d_r.has_value() && !d_y.has_value()) return result;
+    int64_t want = 0;
+    size_t edge = 0;  // only tensors that are there have one
+    for (int i = 0; i < 8; ++i)
+      if (saved[i].defined() && ctx->needs_input_grad(edge++)) want |= 1 << i;
+    auto out = norm_residual_bwd(
+        d_r, d_y, saved[8], saved[0], opt(saved[1]), opt(saved[2]),
+        opt(saved[3]), opt(saved[4]), opt(saved[5]), opt(saved[6]),
+        opt(saved[7]), num, want);
+    bool again = false;  // a graph of the backward pass is asked for
+    for (const auto& g : grads) again |= g.defined() && g.requires_grad();
+    for (const auto& v : saved) again |= v.defined() && v.requires_grad();
+    if (again && at::GradMode::is_enabled()) {
+      auto error = std::make_shared<torch::autograd::DelayedError>(
+          "norm_residual has no second derivatives", (int64_t)out.size());
+      out = (*error)(std::move(out));
+    }
+    std::copy(out.begin(), out.end(), result.begin());
+    return result;
+  }
+};
+
+// (r or None, y or None), with a backward pass where one may follow
+std::pair<OptTensor, OptTensor> norm_residual(
+    const torch::Tensor& x, const OptTensor& h, const OptTensor& gate,
+    const OptTensor& w1, const OptTensor& b1, const OptTensor& w2,
+    const OptTensor& b2, const OptTensor& scale, double scale_value,
+    int64_t post, int64_t pre, int64_t act, double post_eps, double pre_eps,
+    int64_t type_y) {
+  bool train = x.requires_grad();
+  for (auto* t : {&h, &gate, &w1, &b1, &w2, &b2, &scale})
+    train |= t->has_value() && (*t)->requires_grad();
+  std::pair<OptTensor, OptTensor> out;
+  if (train && at::GradMode::is_enabled()) {
+    auto got = NormResidual::apply(x, h, gate, w1, b1, w2, b2, scale,
+                                   scale_value, post, pre, act, post_eps,
+                                   pre_eps, type_y);
+    size_t at = 0;
+    if (h.has_value()) out.first = got.at(at++);
+    if (pre != NORM_NONE) out.second = got.at(at++);
+  } else {
+    const NormNumbers num{scale_value, post_eps, pre_eps, post,
+                          pre,         act,      type_y};
+    auto got = norm_residual_fwd(x, h, gate, w1, b1, w2, b2, scale, num,
+                                 false);
+    if (got[0].defined()) out.first = got[0];
+    if (got[1].defined()) out.second = got[1];
   }
   return out;
 }
@@ -1191,8 +1296,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("multi_tensor_sgd", &multi_tensor_sgd);
   mod.def("ema_flat", &ema_flat);
   mod.def("grad_norm", &grad_norm);
-  mod.def("norm_residual_fwd", &norm_residual_fwd);
-  mod.def("norm_residual_bwd", &norm_residual_bwd);
+  mod.def("norm_residual", &norm_residual);
   mod.def("adamw_step", &adamw_step);
   mod.def("adamw8bit_values", [](const TensorList& m, const TensorList& v,
                                  const TensorList& s, py::object dtype) {

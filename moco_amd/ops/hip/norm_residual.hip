@@ -25,82 +25,141 @@
 // memory once per workgroup, and a second kernel adds those: no atomics, the
 // same bits every time.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "launchers.h"
 
 namespace {
 
-constexpr int V = 8;        // neighbouring elements of a thread
 constexpr int BLOCK = 256;  // threads of a workgroup, at least
+#ifndef NORM_FWD_THREADS
+#define NORM_FWD_THREADS (256 * 1024)
+#endif
 
-template <typename T>
+// V elements as they lie in memory: registers hold whole words until an
+// element is used, so that several loads are on their way at once
+template <typename T, int V>
 struct Raw {
-  T v[V];
+  static constexpr int N = V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1;
+  uint32_t w[N];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __bf16>::value) {
+      return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    } else {
+      const uint16_t u = (uint16_t)(i % 2 ? w[i / 2] >> 16 : w[i / 2]);
+      return (float)__builtin_bit_cast(_Float16, u);
+    }
+  }
 };
 
-// the first n (<= 0: none) of V elements, zeros behind; only the element's
-// own alignment is assumed
-template <typename T>
-__device__ __forceinline__ Raw<T> load_raw(const void* base, int64_t off,
-                                           int n) {
-  Raw<T> r;
-  const T* p = (const T*)base + off;
-  if (n >= V) {
-    __builtin_memcpy(&r, p, sizeof(r));
+// The V neighbouring elements that a thread has of a row.  Where the width is
+// no multiple of V the last thread's begin early enough to end with the row:
+// it then has `skip` elements in common with its neighbour, computes and
+// stores the same values for them, and leaves them out of row sums.  So every
+// access is a whole vector (of the element's own alignment).  A thread that
+// has none (skip = V) reads the row's first, and stores nothing.
+template <int V>
+struct Cols {
+  uint32_t col;
+  int skip;
+  __device__ __forceinline__ void set(int c0, int width, bool row = true) {
+    const bool live = row && c0 < width;
+    const int c = min(c0, width - V);
+    col = live ? c : 0;
+    skip = live ? c0 - c : V;
+  }
+  __device__ __forceinline__ bool live() const { return skip < V; }
+};
+
+// off (to the row) is the same for a wave: it stays in scalar registers, and
+// one 32-bit offset serves all arrays of a type
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const void* base, int64_t off,
+                                              const Cols<V>& c,
+                                              bool wanted = true) {
+  Raw<T, V> r;
+  if (wanted) {
+    const char* p = (const char*)base + off * (int64_t)sizeof(T) +
+                    c.col * (uint32_t)sizeof(T);
+    if constexpr (V * sizeof(T) < 4) {
+      uint16_t u;
+      __builtin_memcpy(&u, p, 2);
+      r.w[0] = u;
+    } else {
+      __builtin_memcpy(r.w, p, sizeof(r.w));
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
+    for (int i = 0; i < Raw<T, V>::N; ++i) r.w[i] = 0;
   }
   return r;
 }
 
-template <typename T>
+template <typename T, int V>
 __device__ __forceinline__ void store_f(void* base, int64_t off,
-                                        const float (&f)[V], int n) {
-  Raw<T> r;
-  T* p = (T*)base + off;
+                                        const Cols<V>& c,
+                                        const float (&f)[V]) {
+  T r[V];
+  char* p = (char*)base + off * (int64_t)sizeof(T);
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = (T)f[i];  // to nearest even
-  if (n >= V) {
-    __builtin_memcpy(p, &r, sizeof(r));
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = r.v[i];
-  }
+  for (int i = 0; i < V; ++i) r[i] = (T)f[i];  // to nearest even
+  if (c.live())
+    __builtin_memcpy(p + c.col * (uint32_t)sizeof(T), r, sizeof(r));
 }
 
 // a per-channel vector (fp32 or TH), or a constant
-template <typename TH>
-__device__ __forceinline__ void load_vec(const void* p, bool f32, int col,
-                                         int n, float none, float (&out)[V]) {
+template <typename TH, int V>
+__device__ __forceinline__ void load_vec(const void* p, bool f32,
+                                         const Cols<V>& c, float none,
+                                         float (&out)[V]) {
   if (p == nullptr) {
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = none;
   } else if (f32) {
-    const Raw<float> r = load_raw<float>(p, col, n);
+    const Raw<float, V> r = load_raw<float>(p, 0, c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = r.v[i];
+    for (int i = 0; i < V; ++i) out[i] = r[i];
   } else {
-    const Raw<TH> r = load_raw<TH>(p, col, n);
+    const Raw<TH, V> r = load_raw<TH>(p, 0, c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = (float)r.v[i];
+    for (int i = 0; i < V; ++i) out[i] = r[i];
   }
+}
+
+// Sum over a wave, the same in all lanes: inside rows of 16 lanes by DPP, the
+// four rows through scalar registers.  (Six ds_bpermute steps take some 400
+// cycles of latency, twice or more a row.)
+__device__ __forceinline__ float wave_sum(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(
+        0, __float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  v += dpp(v, std::integral_constant<int, 0xB1>());   // lane ^ 1
+  v += dpp(v, std::integral_constant<int, 0x4E>());   // lane ^ 2
+  v += dpp(v, std::integral_constant<int, 0x141>());  // half row mirrored
+  v += dpp(v, std::integral_constant<int, 0x140>());  // row mirrored
+  const int b = __float_as_int(v);
+  return (__int_as_float(__builtin_amdgcn_readlane(b, 0)) +
+          __int_as_float(__builtin_amdgcn_readlane(b, 16))) +
+         (__int_as_float(__builtin_amdgcn_readlane(b, 32)) +
+          __int_as_float(__builtin_amdgcn_readlane(b, 48)));
 }
 
 // sums of M values over the NT threads of a row, in a fixed order
 template <int NT, int M>
 struct RowSum {
-  static constexpr int WAVES = NT / WAVE;
+  static constexpr int WAVES = NT / WAVE;  // of this row
   // two slots in turn: one barrier a reduction
   float slot[2][M][WAVES > 1 ? WAVES : 1];
 
   __device__ __forceinline__ void operator()(float (&v)[M], int turn) {
 #pragma unroll
-    for (int j = 0; j < M; ++j) v[j] = wave_reduce_sum(v[j]);
+    for (int j = 0; j < M; ++j) v[j] = wave_sum(v[j]);
     if constexpr (WAVES > 1) {
-      const int wave = threadIdx.x / WAVE;
+      const int wave = threadIdx.x / WAVE % WAVES;
       if (threadIdx.x % WAVE == 0)
 #pragma unroll
         for (int j = 0; j < M; ++j) slot[turn & 1][j][wave] = v[j];
@@ -116,36 +175,54 @@ struct RowSum {
   }
 };
 
+// 1 / (1 + exp(-g)) by the hardware's exp2 and reciprocal: off by (2 + |g|) U
+// (the rounding of g log2(e), and an ulp each), an eighth of expf's and a
+// division's instructions
 __device__ __forceinline__ float sigmoid(float g) {
-  return 1.f / (1.f + expf(-g));
+  return __builtin_amdgcn_rcpf(
+      1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f));
 }
 
-__device__ __forceinline__ float act_of(int act, float g) {
-  if (act == NORM_ACT_NONE) return g;
-  const float s = sigmoid(g);
-  return act == NORM_ACT_SILU ? g * s : s;
-}
-
-__device__ __forceinline__ float act_slope(int act, float g) {
-  if (act == NORM_ACT_NONE) return 1.f;
-  const float s = sigmoid(g);
-  return act == NORM_ACT_SILU ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
+// s[] becomes act(g), g[] becomes act'(g)
+template <int V>
+__device__ __forceinline__ void activate(int act, float (&g)[V],
+                                         float (&s)[V]) {
+  if (act == NORM_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float sig = sigmoid(g[i]);
+      s[i] = g[i] * sig;
+      g[i] = sig + s[i] * (1.f - sig);
+    }
+  } else if (act == NORM_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s[i] = sigmoid(g[i]);
+      g[i] = s[i] * (1.f - s[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s[i] = g[i];
+      g[i] = 1.f;
+    }
+  }
 }
 
 // mean (LayerNorm) and 1/std of a row held as f[K][V]
-template <int NT, int K>
+template <int NT, int K, int V, bool LAYER>
 __device__ __forceinline__ void row_stats(const float (&f)[K][V],
-                                          const int (&n)[K], int kind,
+                                          const Cols<V> (&c)[K], int kind,
                                           float inv_c, float eps,
                                           RowSum<NT, 1>& sum, int& turn,
                                           float& mean, float& rstd) {
   float s[1] = {0.f};
   mean = 0.f;
-  if (kind == NORM_LAYER) {
+  if (LAYER && kind == NORM_LAYER) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[0] += f[k][i];  // zeros behind the row
+      for (int i = 0; i < V; ++i) s[0] += i >= c[k].skip ? f[k][i] : 0.f;
     sum(s, turn++);
     mean = s[0] * inv_c;
     s[0] = 0.f;
@@ -154,98 +231,136 @@ __device__ __forceinline__ void row_stats(const float (&f)[K][V],
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float d = i < n[k] ? f[k][i] - mean : 0.f;
+      const float d = i >= c[k].skip ? f[k][i] - mean : 0.f;
       s[0] += d * d;
     }
   sum(s, turn++);
   rstd = rsqrtf(s[0] * inv_c + eps);
 }
 
-template <typename TX, typename TH, int NT, int K>
+// a row's inputs on their way
+template <typename TX, typename TH, int K, int V>
+struct FwdRow {
+  Raw<TX, V> x[K];
+  Raw<TH, V> h[K], g[K];
+  float row_gate;
+
+  __device__ __forceinline__ void load(const NormArgs& a, int64_t row,
+                                       const Cols<V> (&c)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      x[k] = load_raw<TX>(a.x, row * a.ld_x, c[k]);
+      h[k] = load_raw<TH>(a.h, row * a.ld_h, c[k], a.h != nullptr);
+      g[k] = load_raw<TH>(a.gate, row * a.ld_g, c[k],
+                          a.gate_kind == NORM_GATE_FULL);
+    }
+    row_gate = a.gate_kind == NORM_GATE_ROW
+                   ? (float)((const TH*)a.gate)[row * a.ld_g]
+                   : 1.f;
+  }
+};
+
+// LAYER: whether one norm is a LayerNorm.  A workgroup keeps its columns' weights in
+// registers (K = 1) over its rows, and the next row's inputs are on their way
+// while this one's sums are taken.
+template <typename TX, typename TH, int NT, int K, int V, bool LAYER>
 __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_fwd_kernel(
     const NormArgs a) {
   constexpr int GROUPS = NT < BLOCK ? BLOCK / NT : 1;
+  constexpr bool KEEP = K == 1;
   __shared__ RowSum<NT, 1> sums[GROUPS];
-  const int group = threadIdx.x / NT, t = threadIdx.x % NT;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const int t = threadIdx.x % NT;
   RowSum<NT, 1>& sum = sums[group];
   int turn = 0;
   const float inv_c = 1.f / (float)a.width;
-  // several groups share a workgroup only where they are single waves,
-  // which need no barrier
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < a.rows;
-       row += (int64_t)gridDim.x * GROUPS) {
-    int n[K];
-    Raw<TX> x[K];
-    Raw<TH> g[K];
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  // the groups of a workgroup take the same turns (they share barriers); one
+  // that is behind the last row repeats that row and stores nothing
+  int64_t base = (int64_t)blockIdx.x * GROUPS;
+  auto row_of = [&](int64_t b) {
+    return b + group < a.rows ? b + group : a.rows - 1;
+  };
+  Cols<V> c[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) c[k].set((k * NT + t) * V, a.width);
+  FwdRow<TX, TH, K, V> next;
+  next.load(a, row_of(base), c);
+  float w1[K][V], b1[K][V], w2[K][V], b2[K][V], sc[K][V];
+  auto vectors = [&](int k) {
+    load_vec<TH>(a.w1, a.f32 & 1, c[k], 1.f, w1[k]);
+    if (LAYER) load_vec<TH>(a.b1, a.f32 & 2, c[k], 0.f, b1[k]);
+    load_vec<TH>(a.w2, a.f32 & 4, c[k], 1.f, w2[k]);
+    if (LAYER) load_vec<TH>(a.b2, a.f32 & 8, c[k], 0.f, b2[k]);
+    load_vec<TH>(a.scale, a.f32 & 16, c[k], a.scale_value, sc[k]);
+  };
+  if (KEEP) vectors(0);
+  for (; base < a.rows; base += step) {
+    const bool in = base + group < a.rows;
+    const int64_t row = row_of(base);
+    FwdRow<TX, TH, K, V> cur = next;
+    if (base + step < a.rows) next.load(a, row_of(base + step), c);
     float f[K][V];  // h, later r
-  #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (k * NT + t) * V;
-      n[k] = a.width - col;
-      x[k] = load_raw<TX>(a.x, row * a.ld_x + col, n[k]);
-      if (a.h != nullptr) {
-        const Raw<TH> h = load_raw<TH>(a.h, row * a.ld_h + col, n[k]);
-  #pragma unroll
-        for (int i = 0; i < V; ++i) f[k][i] = (float)h.v[i];
-      }
-      if (a.gate_kind == NORM_GATE_FULL)
-        g[k] = load_raw<TH>(a.gate, row * a.ld_g + col, n[k]);
-    }
     if (a.h == nullptr) {
-  #pragma unroll
+#pragma unroll
       for (int k = 0; k < K; ++k)
-  #pragma unroll
-        for (int i = 0; i < V; ++i) f[k][i] = (float)x[k].v[i];
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[k][i] = cur.x[k][i];
     } else {
-      float row_gate = 1.f;
+      float row_slope[1] = {cur.row_gate}, row_act[1] = {1.f};
       if (a.gate_kind == NORM_GATE_ROW)
-        row_gate = act_of(a.act, (float)((const TH*)a.gate)[row * a.ld_g]);
+        activate(a.act, row_slope, row_act);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[k][i] = cur.h[k][i];
       float mean = 0.f, rstd = 1.f;
       if (a.post != NORM_NONE) {
-        row_stats<NT, K>(f, n, a.post, inv_c, a.post_eps, sum, turn, mean,
-                         rstd);
-        if (t == 0 && a.stats != nullptr) {
+        row_stats<NT, K, V, LAYER>(f, c, a.post, inv_c, a.post_eps, sum, turn, mean,
+                            rstd);
+        if (t == 0 && in && a.stats != nullptr) {
           a.stats[row] = mean;
           a.stats[a.rows + row] = rstd;
         }
       }
-  #pragma unroll
+#pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int col = (k * NT + t) * V;
-        float w[V], b[V], s[V];
-        load_vec<TH>(a.w1, a.f32 & 1, col, n[k], 1.f, w);
-        load_vec<TH>(a.b1, a.f32 & 2, col, n[k], 0.f, b);
-        load_vec<TH>(a.scale, a.f32 & 16, col, n[k], a.scale_value, s);
-  #pragma unroll
+        if (!KEEP) vectors(k);
+#pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float hat = (f[k][i] - mean) * rstd;
-          const float ga = a.gate_kind == NORM_GATE_FULL
-                               ? act_of(a.act, (float)g[k].v[i])
-                               : row_gate;
-          f[k][i] = (float)x[k].v[i] + s[i] * ga * (hat * w[i] + b[i]);
-          if (i >= n[k]) f[k][i] = 0.f;
+          f[k][i] = (LAYER ? f[k][i] - mean : f[k][i]) * (rstd * w1[k][i]);
+          if (LAYER) f[k][i] += b1[k][i];
         }
-        if (a.r != nullptr)
-          store_f<TX>(a.r, row * a.width + col, f[k], n[k]);
+        float act[V], slope[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) act[i] = row_act[0];
+        if (a.gate_kind == NORM_GATE_FULL) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) slope[i] = cur.g[k][i];
+          activate(a.act, slope, act);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          f[k][i] = cur.x[k][i] + sc[k][i] * act[i] * f[k][i];
+        if (in) store_f<TX>(a.r, row * a.width, c[k], f[k]);
       }
     }
     if (a.pre == NORM_NONE) continue;
     float mean, rstd;
-    row_stats<NT, K>(f, n, a.pre, inv_c, a.pre_eps, sum, turn, mean, rstd);
-    if (t == 0 && a.stats != nullptr) {
+    row_stats<NT, K, V, LAYER>(f, c, a.pre, inv_c, a.pre_eps, sum, turn, mean, rstd);
+    if (t == 0 && in && a.stats != nullptr) {
       a.stats[2 * a.rows + row] = mean;
       a.stats[3 * a.rows + row] = rstd;
     }
-  #pragma unroll
+#pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * NT + t) * V;
-      float w[V], b[V];
-      load_vec<TH>(a.w2, a.f32 & 4, col, n[k], 1.f, w);
-      load_vec<TH>(a.b2, a.f32 & 8, col, n[k], 0.f, b);
-  #pragma unroll
-      for (int i = 0; i < V; ++i)
-        f[k][i] = (f[k][i] - mean) * rstd * w[i] + b[i];
-      store_f<TH>(a.y, row * a.width + col, f[k], n[k]);
+      if (!KEEP) vectors(k);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        f[k][i] = (LAYER ? f[k][i] - mean : f[k][i]) * (rstd * w2[k][i]);
+        if (LAYER) f[k][i] += b2[k][i];
+      }
+      if (in) store_f<TH>(a.y, row * a.width, c[k], f[k]);
     }
   }
 }
@@ -254,17 +369,64 @@ __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_fwd_kernel(
 // dw2, db2, dscale.
 constexpr int VECS = 5;
 
-template <typename TX, typename TH, int NT, int K>
-__global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_bwd_kernel(
-    const NormArgs a, const NormGrads o) {
+// LAYER: whether one norm is a LayerNorm (or has a bias).  What bounds this
+// pass after memory is the number of vector instructions, some 50 an element,
+// and registers, which bound how many rows are on their way per CU.  So hats
+// and weighted values are made again rather than kept, and the weights are
+// read from LDS (K = 1), where a workgroup puts them once.
+template <typename TX, typename TH, int NT, int K, int V, bool LAYER>
+__global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT,
+                             LAYER && NT < 1024 ? 3 : 4) void
+norm_bwd_kernel(const NormArgs a, const NormGrads o) {
   constexpr int GROUPS = NT < BLOCK ? BLOCK / NT : 1;
+  constexpr bool KEEP = K == 1;
+  constexpr int KEPT = LAYER ? 4 : 3;  // w1, scale, w2, b1
   __shared__ RowSum<NT, 2> sums2[GROUPS];
   __shared__ RowSum<NT, 3> sums3[GROUPS];
-  __shared__ float across[GROUPS > 1 ? GROUPS * NT * K * V : 1];
-  const int group = threadIdx.x / NT, t = threadIdx.x % NT;
+  // [vector][four elements][thread]: neighbouring threads' reads of 16 bytes
+  // lie side by side
+  constexpr int Q = V >= 4 ? V / 4 : 1, W = V / Q;
+  __shared__ float kept[KEEP ? KEPT : 1][KEEP ? Q : 1][KEEP ? NT : 1][W];
+  __shared__ float across[GROUPS > 1 ? GROUPS : 1]
+                         [GROUPS > 1 ? NT * K * V : 1];
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const int t = threadIdx.x % NT;
   RowSum<NT, 2>& sum2 = sums2[group];
   RowSum<NT, 3>& sum3 = sums3[group];
   const float inv_c = 1.f / (float)a.width;
+  const bool full = a.gate_kind == NORM_GATE_FULL;
+  const bool per_row = a.gate_kind == NORM_GATE_ROW;
+  Cols<V> c[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) c[k].set((k * NT + t) * V, a.width);
+  auto fetch = [&](int which, int k, float (&v)[V]) {
+    switch (which) {
+      case 0: load_vec<TH>(a.w1, a.f32 & 1, c[k], 1.f, v); break;
+      case 1: load_vec<TH>(a.scale, a.f32 & 16, c[k], a.scale_value, v); break;
+      case 2: load_vec<TH>(a.w2, a.f32 & 4, c[k], 1.f, v); break;
+      default: load_vec<TH>(a.b1, a.f32 & 2, c[k], 0.f, v); break;
+    }
+  };
+  if constexpr (KEEP) {
+    if (group == 0) {
+#pragma unroll
+      for (int j = 0; j < KEPT; ++j) {
+        float v[V];
+        fetch(j, 0, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) kept[j][i / W][t][i % W] = v[i];
+      }
+    }
+    __syncthreads();
+  }
+  auto vec = [&](int which, int k, float (&v)[V]) {
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = kept[which][i / W][t][i % W];
+    } else {
+      fetch(which, k, v);
+    }
+  };
   float acc[VECS][K][V];
 #pragma unroll
   for (int j = 0; j < VECS; ++j)
@@ -272,135 +434,161 @@ __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_bwd_kernel(
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[j][k][i] = 0.f;
-  int n[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) n[k] = a.width - (k * NT + t) * V;
   int turn = 0;
-  // the same number of turns for all threads of a group; several groups
-  // share a workgroup only where they need no barrier
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < a.rows;
-       row += (int64_t)gridDim.x * GROUPS, ++turn) {
-    Raw<TX> x[K], dr[K];
-    Raw<TH> h[K], g[K], dy[K];
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < a.rows;
+       base += (int64_t)gridDim.x * GROUPS, ++turn) {
+    const bool in = base + group < a.rows;
+    const int64_t row = in ? base + group : a.rows - 1;
+    Raw<TX, V> x[K], dr[K];
+    Raw<TH, V> h[K], g[K], dy[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * NT + t) * V;
-      x[k] = load_raw<TX>(a.x, row * a.ld_x + col, n[k]);
-      if (a.h != nullptr)
-        h[k] = load_raw<TH>(a.h, row * a.ld_h + col, n[k]);
-      if (a.gate_kind == NORM_GATE_FULL)
-        g[k] = load_raw<TH>(a.gate, row * a.ld_g + col, n[k]);
-      dr[k] = load_raw<TX>(o.d_r, row * a.width + col,
-                           o.d_r != nullptr ? n[k] : 0);
-      dy[k] = load_raw<TH>(o.d_y, row * a.width + col,
-                           o.d_y != nullptr ? n[k] : 0);
+      x[k] = load_raw<TX>(a.x, row * a.ld_x, c[k], o.d_y != nullptr);
+      h[k] = load_raw<TH>(a.h, row * a.ld_h, c[k], a.h != nullptr);
+      g[k] = load_raw<TH>(a.gate, row * a.ld_g, c[k], full);
+      // zeros behind the last row: nothing is added to the column sums
+      dr[k] = load_raw<TX>(o.d_r, row * a.width, c[k],
+                           o.d_r != nullptr && in);
+      dy[k] = load_raw<TH>(o.d_y, row * a.width, c[k],
+                           o.d_y != nullptr && in);
     }
     float mean_h = 0.f, rstd_h = 1.f, mean_r = 0.f, rstd_r = 0.f;
     if (a.h != nullptr && a.post != NORM_NONE) {
-      mean_h = a.stats[row];
+      if (LAYER) mean_h = a.stats[row];
       rstd_h = a.stats[a.rows + row];
     }
     if (o.d_y != nullptr) {
-      mean_r = a.stats[2 * a.rows + row];
+      if (LAYER) mean_r = a.stats[2 * a.rows + row];
       rstd_r = a.stats[3 * a.rows + row];
     }
-    float row_raw = 0.f, row_gate = 1.f;
-    if (a.gate_kind == NORM_GATE_ROW) {
-      row_raw = (float)((const TH*)a.gate)[row * a.ld_g];
-      row_gate = act_of(a.act, row_raw);
+    float row_act[1] = {1.f}, row_slope[1] = {0.f};
+    if (per_row) {
+      row_slope[0] = (float)((const TH*)a.gate)[row * a.ld_g];
+      activate(a.act, row_slope, row_act);
     }
-    // n = hhat w1 + b1 and r, then the norm before the next block
-    float nf[K][V], hat[K][V], ga[K][V], d[K][V];
-    float p[2] = {0.f, 0.f};
+    float d[K][V], act[K][V], slope[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * NT + t) * V;
-      float w[V], b[V], s[V];
-      if (a.h != nullptr) {
-        load_vec<TH>(a.w1, a.f32 & 1, col, n[k], 1.f, w);
-        load_vec<TH>(a.b1, a.f32 & 2, col, n[k], 0.f, b);
-        load_vec<TH>(a.scale, a.f32 & 16, col, n[k], a.scale_value, s);
-      }
-      float w2[V];
-      load_vec<TH>(a.w2, a.f32 & 4, col, n[k], 1.f, w2);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float r = (float)x[k].v[i];
-        if (a.h != nullptr) {
-          hat[k][i] = ((float)h[k].v[i] - mean_h) * rstd_h;
-          nf[k][i] = hat[k][i] * w[i] + b[i];
-          ga[k][i] = a.gate_kind == NORM_GATE_FULL
-                         ? act_of(a.act, (float)g[k].v[i])
-                         : row_gate;
-          r += s[i] * ga[k][i] * nf[k][i];
-        }
-        const float rhat =
-            i < n[k] && o.d_y != nullptr ? (r - mean_r) * rstd_r : 0.f;
-        const float dyf = (float)dy[k].v[i];
-        const float tt = dyf * w2[i];
-        acc[2][k][i] += dyf * rhat;
-        acc[3][k][i] += dyf;
-        p[0] += tt * rhat;
-        p[1] += tt;
-        d[k][i] = rhat;  // until the sums are there
+      for (int i = 0; i < V; ++i) act[k][i] = row_act[0], slope[k][i] = 1.f;
+      if (full) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) slope[k][i] = g[k][i];
+        activate(a.act, slope[k], act[k]);
       }
     }
+    auto hat_h = [&](int k, int i) {
+      return (LAYER ? h[k][i] - mean_h : h[k][i]) * rstd_h;
+    };
+    // the norm before the next block: its row sums need r
+    float p[2] = {0.f, 0.f};
     if (o.d_y != nullptr) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float v[V];
+        if (a.h != nullptr) {
+          vec(0, k, v);
+#pragma unroll
+          for (int i = 0; i < V; ++i) d[k][i] = hat_h(k, i) * v[i];
+          if (LAYER) {
+            vec(3, k, v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) d[k][i] += v[i];
+          }
+          vec(1, k, v);
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            d[k][i] = x[k][i] + v[i] * act[k][i] * d[k][i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) d[k][i] = x[k][i];
+        }
+        vec(2, k, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          d[k][i] = (LAYER ? d[k][i] - mean_r : d[k][i]) * rstd_r;  // hat
+          const float tt = i >= c[k].skip ? dy[k][i] * v[i] : 0.f;
+          acc[2][k][i] += dy[k][i] * d[k][i];
+          if (LAYER) acc[3][k][i] += dy[k][i];
+          p[0] += tt * d[k][i];
+          if (LAYER) p[1] += tt;
+        }
+      }
       sum2(p, turn);
       p[0] *= inv_c;
-      p[1] = a.pre == NORM_LAYER ? p[1] * inv_c : 0.f;
+      p[1] = LAYER && a.pre == NORM_LAYER ? p[1] * inv_c : 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float v[V];
+        vec(2, k, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float back = dy[k][i] * v[i] - d[k][i] * p[0];
+          d[k][i] = dr[k][i] + rstd_r * (LAYER ? back - p[1] : back);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[k][i] = dr[k][i];
     }
+    if (o.d_x != nullptr && in) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        store_f<TX>(o.d_x, row * a.width, c[k], d[k]);
+    }
+    if (a.h == nullptr) continue;
+    // the gate, the scale and the norm after the block
     float q[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * NT + t) * V;
-      float w2[V], w[V], s[V];
-      load_vec<TH>(a.w2, a.f32 & 4, col, n[k], 1.f, w2);
+      float w[V], s[V], nf[V];
+      vec(0, k, w);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float dn =
-            rstd_r * ((float)dy[k].v[i] * w2[i] - p[1] - d[k][i] * p[0]);
-        d[k][i] = (float)dr[k].v[i] + (o.d_y != nullptr ? dn : 0.f);
+      for (int i = 0; i < V; ++i) nf[i] = hat_h(k, i) * w[i];
+      if (LAYER) {
+        float b[V];
+        vec(3, k, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) nf[i] += b[i];
       }
-      if (o.d_x != nullptr)
-        store_f<TX>(o.d_x, row * a.width + col, d[k], n[k]);
-      if (a.h == nullptr) continue;
-      load_vec<TH>(a.w1, a.f32 & 1, col, n[k], 1.f, w);
-      load_vec<TH>(a.scale, a.f32 & 16, col, n[k], a.scale_value, s);
-      float dg[V];
+      vec(1, k, s);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        if (i >= n[k]) d[k][i] = 0.f;
-        const float dsn = d[k][i] * nf[k][i];
-        acc[4][k][i] += dsn * ga[k][i];
-        const float da = dsn * s[i];
-        q[2] += da;
-        if (a.gate_kind == NORM_GATE_FULL)
-          dg[i] = da * act_slope(a.act, (float)g[k].v[i]);
-        const float dn = d[k][i] * s[i] * ga[k][i];
-        acc[0][k][i] += dn * hat[k][i];
-        acc[1][k][i] += dn;
+        const float dsn = d[k][i] * nf[i];
+        acc[4][k][i] += dsn * act[k][i];
+        slope[k][i] *= dsn * s[i];
+        const float dn = d[k][i] * (s[i] * act[k][i]);
+        acc[0][k][i] += dn * hat_h(k, i);
+        if (LAYER) acc[1][k][i] += dn;
         d[k][i] = dn * w[i];  // t1 from here on
-        q[0] += d[k][i] * hat[k][i];
-        q[1] += d[k][i];
+        const float t1 = i >= c[k].skip ? d[k][i] : 0.f;
+        q[0] += t1 * hat_h(k, i);
+        if (LAYER) q[1] += t1;
       }
-      if (a.gate_kind == NORM_GATE_FULL && o.d_gate != nullptr)
-        store_f<TH>(o.d_gate, row * a.width + col, dg, n[k]);
+      if (full && o.d_gate != nullptr && in)
+        store_f<TH>(o.d_gate, row * a.width, c[k], slope[k]);
+      if (per_row) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          q[2] += i >= c[k].skip ? slope[k][i] : 0.f;
+      }
     }
-    if (a.h == nullptr) continue;
-    if (a.post != NORM_NONE || a.gate_kind == NORM_GATE_ROW) sum3(q, turn);
-    if (a.gate_kind == NORM_GATE_ROW && o.d_gate != nullptr && t == 0)
-      ((TH*)o.d_gate)[row] = (TH)(q[2] * act_slope(a.act, row_raw));
-    if (o.d_h == nullptr) continue;
+    if (a.post != NORM_NONE || per_row) sum3(q, turn);
+    if (per_row && o.d_gate != nullptr && t == 0 && in)
+      ((TH*)o.d_gate)[row] = (TH)(q[2] * row_slope[0]);
+    if (o.d_h == nullptr || !in) continue;
     const float m1 = a.post != NORM_NONE ? q[0] * inv_c : 0.f;
-    const float m0 = a.post == NORM_LAYER ? q[1] * inv_c : 0.f;
+    const float m0 = LAYER && a.post == NORM_LAYER ? q[1] * inv_c : 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * NT + t) * V;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        d[k][i] = rstd_h * (d[k][i] - m0 - hat[k][i] * m1);
-      store_f<TH>(o.d_h, row * a.width + col, d[k], n[k]);
+      for (int i = 0; i < V; ++i) {
+        const float back = d[k][i] - hat_h(k, i) * m1;
+        d[k][i] = rstd_h * (LAYER ? back - m0 : back);
+      }
+      store_f<TH>(o.d_h, row * a.width, c[k], d[k]);
     }
   }
   // the workgroup's column sums: its groups' are added in LDS first
@@ -412,20 +600,17 @@ __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_bwd_kernel(
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          across[((group * K + k) * NT + t) * V + i] = acc[j][k][i];
+        store_f<float>(across[group], 0, c[k], acc[j][k]);
       __syncthreads();
-      for (int c = threadIdx.x; c < a.width; c += BLOCK) {
+      for (int i = threadIdx.x; i < a.width; i += BLOCK) {
         float s = 0.f;
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr) s += across[gr * K * NT * V + c];
-        out[c] = s;
+        for (int gr = 0; gr < GROUPS; ++gr) s += across[gr][i];
+        out[i] = s;
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        store_f<float>(out, (k * NT + t) * V, acc[j][k], n[k]);
+      for (int k = 0; k < K; ++k) store_f<float>(out, 0, c[k], acc[j][k]);
     }
   }
 }
@@ -455,29 +640,39 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(
   }
 }
 
-template <typename TX, typename TH, int NT, int K>
+template <typename TX, typename TH, int NT, int K, int V>
 void go(hipStream_t s, const NormArgs& a, const NormGrads* o, int blocks) {
   constexpr int GROUPS = NT < BLOCK ? BLOCK / NT : 1;
   constexpr int THREADS = NT < BLOCK ? BLOCK : NT;
+  const bool layer = a.post == NORM_LAYER || a.pre == NORM_LAYER;
   if (o == nullptr) {
-    // a grid holds fewer than 2^32 threads
     const int64_t grid = std::min<int64_t>((a.rows + GROUPS - 1) / GROUPS,
-                                           1 << 20);
-    norm_fwd_kernel<TX, TH, NT, K><<<dim3((unsigned)grid), THREADS, 0, s>>>(a);
+                                           NORM_FWD_THREADS / THREADS);
+    if (layer)
+      norm_fwd_kernel<TX, TH, NT, K, V, true>
+          <<<dim3((unsigned)grid), THREADS, 0, s>>>(a);
+    else
+      norm_fwd_kernel<TX, TH, NT, K, V, false>
+          <<<dim3((unsigned)grid), THREADS, 0, s>>>(a);
+  } else if (layer) {
+    norm_bwd_kernel<TX, TH, NT, K, V, true>
+        <<<dim3(blocks), THREADS, 0, s>>>(a, *o);
   } else {
-    norm_bwd_kernel<TX, TH, NT, K><<<dim3(blocks), THREADS, 0, s>>>(a, *o);
+    norm_bwd_kernel<TX, TH, NT, K, V, false>
+        <<<dim3(blocks), THREADS, 0, s>>>(a, *o);
   }
 }
 
 template <typename TX, typename TH>
 int go_width(hipStream_t s, const NormArgs& a, const NormGrads* o,
              int blocks) {
-  if (a.width <= 512) go<TX, TH, 64, 1>(s, a, o, blocks);
-  else if (a.width <= 1024) go<TX, TH, 64, 2>(s, a, o, blocks);
-  else if (a.width <= 2048) go<TX, TH, 256, 1>(s, a, o, blocks);
-  else if (a.width <= 4096) go<TX, TH, 256, 2>(s, a, o, blocks);
-  else if (a.width <= 8192) go<TX, TH, 1024, 1>(s, a, o, blocks);
-  else if (a.width <= NORM_MAX_WIDTH) go<TX, TH, 1024, 2>(s, a, o, blocks);
+  if (a.width < 8) go<TX, TH, 64, 1, 1>(s, a, o, blocks);
+  else if (a.width <= 512) go<TX, TH, 64, 1, 8>(s, a, o, blocks);
+  else if (a.width <= 1024) go<TX, TH, 128, 1, 8>(s, a, o, blocks);
+  else if (a.width <= 2048) go<TX, TH, 256, 1, 8>(s, a, o, blocks);
+  else if (a.width <= 4096) go<TX, TH, 512, 1, 8>(s, a, o, blocks);
+  else if (a.width <= 8192) go<TX, TH, 1024, 1, 8>(s, a, o, blocks);
+  else if (a.width <= NORM_MAX_WIDTH) go<TX, TH, 1024, 2, 8>(s, a, o, blocks);
   else return (int)hipErrorInvalidValue;
   HIP_CHECK_LAST();
   return 0;
@@ -503,7 +698,7 @@ extern "C" int launch_norm_fwd(void* stream, const NormArgs* a) {
 }
 
 extern "C" int norm_bwd_blocks(int64_t rows, int64_t width) {
-  const int64_t groups = width <= 1024 ? BLOCK / WAVE : 1;
+  const int64_t groups = width <= 512 ? 4 : width <= 1024 ? 2 : 1;
   const int64_t most = (rows + groups - 1) / groups;
   return (int)(most < 512 ? most : 512);
 }

@@ -3,7 +3,9 @@ scale, as one op: where one block ends and the next begins.
 
 Beside bn_act (bn.py), which does the same for convolution blocks: there the
 norm is over the batch, here over the last dimension (RMSNorm, LayerNorm).
-GPU path: ops/hip/norm_residual.hip.  The reference has batch norms only.
+GPU path: ops/hip/norm_residual.hip, with its autograd node in bindings.cpp
+(a node in Python cost some 60 us of host time a call, twice what the kernels
+of a small batch take).  The reference has batch norms only.
 """
 
 from typing import Optional, Tuple, Union
@@ -36,30 +38,6 @@ def _norm_args(mod: Optional[Norm], width: int, which: str):
     if mod.eps is None or not mod.eps >= 0.0:
         raise ValueError(f"{which} needs an eps of its own, got {mod.eps}")
     return kind, mod.weight, bias, mod.eps
-
-
-class _NormResidual(torch.autograd.Function):
-    """Tensors: x, branch, gate, post weight and bias, pre weight and bias,
-    scale."""
-
-    @staticmethod
-    def forward(ctx, numbers, *tensors):
-        r, y, stats = ext().norm_residual_fwd(*tensors, *numbers, True)
-        ctx.save_for_backward(stats, *tensors)
-        ctx.numbers = numbers
-        ctx.set_materialize_grads(False)
-        return r, y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_r, d_y):
-        if d_r is None and d_y is None:
-            return (None,) * 9
-        want = sum(1 << i for i, w in enumerate(ctx.needs_input_grad[1:])
-                   if w)
-        stats, *tensors = ctx.saved_tensors
-        return (None, *ext().norm_residual_bwd(d_r, d_y, stats, *tensors,
-                                               *ctx.numbers, want))
 
 
 def _plain_norm(x, kind, weight, bias, eps):
@@ -175,13 +153,9 @@ def norm_residual(x: torch.Tensor, branch: Optional[torch.Tensor] = None, *,
         if block_type not in _TYPES:
             raise TypeError(f"on the GPU the block's type is float32, "
                             f"bfloat16 or float16, got {block_type}")
-        numbers = (scale_value, post_kind, pre_kind, _ACTS[gate_act], eps1,
-                   eps2, _TYPES[block_type])
-        if torch.is_grad_enabled() and any(
-                t is not None and t.requires_grad for t in tensors):
-            r, y = _NormResidual.apply(numbers, *tensors)
-        else:
-            r, y, _ = ext().norm_residual_fwd(*tensors, *numbers, False)
+        r, y = ext().norm_residual(
+            *tensors, scale_value, post_kind, pre_kind, _ACTS[gate_act],
+            eps1, eps2, _TYPES[block_type])
     else:
         if block_type not in _TYPES and block_type != torch.float64:
             raise TypeError(f"the block's type must be a float type, got "
