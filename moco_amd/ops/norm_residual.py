@@ -32,12 +32,45 @@ def _norm_args(mod: Optional[Norm], width: int, which: str):
     else:
         raise TypeError(f"{which} must be an nn.RMSNorm or nn.LayerNorm, got "
                         f"{type(mod).__name__}")
-    if tuple(mod.normalized_shape) != (width,):
-        raise ValueError(f"{which} normalizes {tuple(mod.normalized_shape)}, "
-                         f"the last dimension is {width}")
+    if mod.normalized_shape != (width,):
+        raise ValueError(f"{which} normalizes {mod.normalized_shape}, the "
+                         f"last dimension is {width}")
     if mod.eps is None or not mod.eps >= 0.0:
         raise ValueError(f"{which} needs an eps of its own, got {mod.eps}")
     return kind, mod.weight, bias, mod.eps
+
+
+def _check_tensors(x, branch, gate, vectors, block_type):
+    """What the GPU's entry point checks by itself."""
+    width = x.shape[-1]
+    if block_type not in _TYPES and block_type != torch.float64:
+        raise TypeError(f"the block's type must be a float type, got "
+                        f"{block_type}")
+    if branch is not None and branch.shape != x.shape:
+        raise ValueError(f"branch is {tuple(branch.shape)}, x "
+                         f"{tuple(x.shape)}")
+    if x.dtype not in (torch.float32, block_type):
+        raise TypeError(f"x must be float32 or of the block's type, got "
+                        f"{x.dtype} with {block_type}")
+    if gate is not None:
+        if gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or \
+                gate.shape[-1] not in (1, width):
+            raise ValueError(f"gate must be {tuple(x.shape)} or have 1 as "
+                             f"its last dimension, got {tuple(gate.shape)}")
+        if gate.dtype != block_type:
+            raise TypeError(f"gate is {gate.dtype}, the branch {block_type}")
+    for v in vectors:
+        if v is None:
+            continue
+        if v.shape != (width,):
+            raise ValueError(f"weights, biases and scale must be [{width}], "
+                             f"got {tuple(v.shape)}")
+        if v.dtype not in (torch.float32, block_type):
+            raise TypeError("weights, biases and scale must be float32 or of "
+                            f"the block's type, got {v.dtype}")
+    if any(t is not None and t.device != x.device
+           for t in (branch, gate, *vectors)):
+        raise ValueError("all tensors must be on one device")
 
 
 def _plain_norm(x, kind, weight, bias, eps):
@@ -98,14 +131,17 @@ def norm_residual(x: torch.Tensor, branch: Optional[torch.Tensor] = None, *,
     last dimension is dense, other layouts are copied.  On the GPU width is
     16384 at most.
     """
-    if x.dim() < 1 or x.shape[-1] < 1:
+    width = x.shape[-1] if x.dim() else 0
+    if width < 1:
         raise ValueError(f"x must be [..., width], got {tuple(x.shape)}")
-    width = x.shape[-1]
     post_kind, w1, b1, eps1 = _norm_args(post, width, "post")
     pre_kind, w2, b2, eps2 = _norm_args(pre, width, "pre")
-    if gate_act not in _ACTS:
+    act = _ACTS.get(gate_act)
+    if act is None:
         raise ValueError(f"gate_act must be None, 'sigmoid' or 'silu', got "
                          f"{gate_act!r}")
+    if gate is None and act:
+        raise ValueError("gate_act needs a gate")
     if branch is None:
         if post is not None or gate is not None or scale is not None:
             raise ValueError("post, gate and scale need a branch")
@@ -114,52 +150,25 @@ def norm_residual(x: torch.Tensor, branch: Optional[torch.Tensor] = None, *,
         block_type = out_dtype or x.dtype
     else:
         block_type = branch.dtype
-        if out_dtype not in (None, block_type):
+        if out_dtype is not None and out_dtype != block_type:
             raise ValueError("y has the branch's type: out_dtype is for calls "
                              "without one")
-        if branch.shape != x.shape:
-            raise ValueError(f"branch is {tuple(branch.shape)}, x "
-                             f"{tuple(x.shape)}")
-    if gate is None:
-        if gate_act is not None:
-            raise ValueError("gate_act needs a gate")
-    elif gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or \
-            gate.shape[-1] not in (1, width):
-        raise ValueError(f"gate must be {tuple(x.shape)} or have 1 as its "
-                         f"last dimension, got {tuple(gate.shape)}")
     scale_value = 1.0
     if isinstance(scale, torch.Tensor):
         if scale.numel() == 1 and width > 1:
             scale = scale.reshape(1).expand(width)
-        if scale.shape != (width,):
-            raise ValueError(f"scale must be a number or [{width}], got "
-                             f"{tuple(scale.shape)}")
     elif scale is not None:
         scale, scale_value = None, float(scale)
-    if x.dtype not in (torch.float32, block_type):
-        raise TypeError(f"x must be float32 or of the block's type, got "
-                        f"{x.dtype} with {block_type}")
-    if gate is not None and gate.dtype != block_type:
-        raise TypeError(f"gate is {gate.dtype}, the branch {block_type}")
-    tensors = (x, branch, gate, w1, b1, w2, b2, scale)
-    for t in tensors[3:]:
-        if t is not None and t.dtype not in (torch.float32, block_type):
-            raise TypeError("weights, biases and scale must be float32 or of "
-                            f"the block's type, got {t.dtype}")
-    if any(t is not None and t.device != x.device for t in tensors):
-        raise ValueError("all tensors must be on one device")
-
-    if use_hip(x):
-        if block_type not in _TYPES:
+    if x.is_cuda and use_hip(x):  # shapes, types, devices: checked in C++
+        kind = _TYPES.get(block_type)
+        if kind is None:
             raise TypeError(f"on the GPU the block's type is float32, "
                             f"bfloat16 or float16, got {block_type}")
-        r, y = ext().norm_residual(
-            *tensors, scale_value, post_kind, pre_kind, _ACTS[gate_act],
-            eps1, eps2, _TYPES[block_type])
+        r, y = ext().norm_residual(x, branch, gate, w1, b1, w2, b2, scale,
+                                   scale_value, post_kind, pre_kind, act,
+                                   eps1, eps2, kind)
     else:
-        if block_type not in _TYPES and block_type != torch.float64:
-            raise TypeError(f"the block's type must be a float type, got "
-                            f"{block_type}")
-        r, y = _plain(*tensors, scale_value, post_kind, pre_kind,
-                      _ACTS[gate_act], eps1, eps2, block_type)
+        _check_tensors(x, branch, gate, (w1, b1, w2, b2, scale), block_type)
+        r, y = _plain(x, branch, gate, w1, b1, w2, b2, scale, scale_value,
+                      post_kind, pre_kind, act, eps1, eps2, block_type)
     return (x if branch is None else r), y
