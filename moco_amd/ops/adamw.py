@@ -170,6 +170,8 @@ def _encode(m: torch.Tensor, r: torch.Tensor, key: Optional[int]):
     m, r = _blocks(m), _blocks(r)
     sm = m.abs().amax(1, keepdim=True).clamp_min(_TINY) * (1 / _TOP_M)
     sr = r.amax(1, keepdim=True).clamp_min(_TINY) * (1 / _TOP_R)
+    # an infinity in a block makes all of it a NaN
+    sm, sr = (t.masked_fill(t == math.inf, math.nan) for t in (sm, sr))
     mc = (m * sm.reciprocal()).clamp(-_TOP_M, _TOP_M).to(torch.float8_e4m3fn)
     q = r * sr.reciprocal()
     dither = 1 << 18 if key is None else \
@@ -382,8 +384,6 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _init_state(self, p, bits):
         state = self.state[p]
-        if state:
-            return state
         if not _is_dense(p):
             raise ValueError("FusedAdamW needs dense parameters, got strides "
                              f"{p.stride()} for shape {tuple(p.shape)}")
@@ -412,7 +412,7 @@ class FusedAdamW(torch.optim.Optimizer):
             raise RuntimeError("FusedAdamW.step() counts its steps on the "
                                "host and cannot be captured into a graph")
         # lists of equal step count, per group and kind of state
-        buckets, every_grad = {}, []
+        buckets, every_grad, last = {}, [], None
         for gi, group in enumerate(self.param_groups):
             for p in group["params"]:
                 g = p.grad
@@ -420,16 +420,21 @@ class FusedAdamW(torch.optim.Optimizer):
                     continue
                 if g.is_sparse:
                     raise ValueError("sparse gradients are not supported")
-                state = self._init_state(p, group["state_bits"])
-                if not _same_layout(p, g):
+                state = self.state[p] or self._init_state(
+                    p, group["state_bits"])
+                if g.stride() != p.stride() and not _same_layout(p, g):
                     g = torch.empty_like(p).copy_(g)
                 scales = state.get("scales")
-                lists = buckets.setdefault(
-                    (gi, state["step"], scales is not None),
-                    ([], [], [], [], []))
-                for lst, t in zip(lists, (p, g, state["exp_avg"],
-                                          state["exp_avg_sq"], scales)):
-                    lst.append(t)
+                key = (gi, state["step"], scales is not None)
+                if key != last:
+                    last = key
+                    ps, gs, ms, vs, ss = buckets.setdefault(
+                        key, ([], [], [], [], []))
+                ps.append(p)
+                gs.append(g)
+                ms.append(state["exp_avg"])
+                vs.append(state["exp_avg_sq"])
+                ss.append(scales)
                 every_grad.append(g)
         norm = None
         if self.max_grad_norm is not None and every_grad:

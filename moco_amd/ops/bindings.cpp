@@ -297,24 +297,49 @@ void check_disjoint(std::vector<Range>& r) {
   }
 }
 
-// fills tables of one dtype and hands each to `launch`
+// chunks of n elements, and how many the last one has
+int64_t chunks_of(int64_t n, uint16_t& tail) {
+  const int64_t chunks = (n + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
+  tail = (uint16_t)(n - (chunks - 1) * ADAMW_CHUNK);
+  return chunks;
+}
+
+// a grid holds fewer than 2^32 threads, 256 of them a chunk
+constexpr int64_t MOST_CHUNKS = ((int64_t)1 << 24) - 1;
+
+// room for a tensor in a table; hands the table to `launch` first if needed
+template <typename Table, typename F>
+int next_slot(Table& tab, int most, int64_t chunks, const F& launch) {
+  TORCH_CHECK_VALUE(chunks <= MOST_CHUNKS, "a tensor of over ",
+                    MOST_CHUNKS * ADAMW_CHUNK, " elements is too large");
+  if (tab.count == most || tab.chunks + chunks > MOST_CHUNKS) {
+    launch(tab);
+    tab.count = 0, tab.chunks = 0;
+  }
+  tab.first[tab.count] = tab.chunks;
+  tab.chunks += (uint32_t)chunks;
+  return tab.count++;
+}
+
+// fills AdamwTables of one dtype and hands each to `launch`
 template <typename F>
 struct TableFiller {
   AdamwTable tab;
   F launch;
-  explicit TableFiller(F f) : launch(f) { tab.count = 0, tab.chunks = 0; }
+  explicit TableFiller(F f) : launch(f) {
+    tab.count = 0, tab.chunks = 0, tab.list_base = 0;
+  }
   void add(void* p, const void* g, void* m, void* v, void* s, int64_t n,
-           uint32_t key) {
-    const int64_t chunks = (n + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
-    // a grid holds fewer than 2^32 threads, 256 of them a chunk
-    constexpr int64_t MOST = ((int64_t)1 << 24) - 1;
-    TORCH_CHECK_VALUE(chunks <= MOST, "a tensor of ", n,
-                      " elements is too large");
-    if (tab.count == ADAMW_TENSORS || tab.chunks + chunks > MOST) flush();
-    const int i = tab.count++;
+           size_t number) {
+    if ((number >> 16 << 16) != tab.list_base) {
+      flush();
+      tab.list_base = (uint32_t)(number >> 16 << 16);
+    }
+    uint16_t tail;
+    const int64_t chunks = chunks_of(n, tail);
+    const int i = next_slot(tab, ADAMW_TENSORS, chunks, launch);
     tab.p[i] = p, tab.g[i] = g, tab.m[i] = m, tab.v[i] = v, tab.s[i] = s;
-    tab.n[i] = n, tab.first[i] = tab.chunks, tab.key[i] = key;
-    tab.chunks += (uint32_t)chunks;
+    tab.tail[i] = tail, tab.number[i] = (uint16_t)number;
   }
   void flush() {
     if (tab.count) launch(tab);
@@ -326,28 +351,38 @@ struct TableFiller {
 torch::Tensor grad_norm_checked(const TensorList& grads) {
   auto opts = grads[0].options().dtype(torch::kFloat32).layout(torch::kStrided);
   auto out = torch::empty({}, opts);
-  constexpr int BLOCKS = 1024;
-  // a launch takes ADAMW_TENSORS tensors of one dtype: at most this many
-  const int64_t launches = (int64_t)grads.size() / ADAMW_TENSORS + 3;
+  // workgroups of a launch at most: 8 per CU, which fill it with loads
+  constexpr int64_t BLOCKS = 2048;
+  // a launch takes GRAD_TENSORS tensors of one dtype or MOST_CHUNKS chunks
+  int64_t launches = (int64_t)grads.size() / GRAD_TENSORS + 3, elements = 0;
+  for (const auto& g : grads) elements += g.numel();
+  launches += 2 * (elements / ADAMW_CHUNK + (int64_t)grads.size()) /
+              MOST_CHUNKS;
   auto partial = torch::empty({launches * BLOCKS},
                               opts.dtype(torch::kFloat64));
   double* at = partial.data_ptr<double>();
-  int used = 0;
+  int64_t used = 0;
   for (int dtype = 0; dtype < 3; ++dtype) {
-    auto go = [&](const AdamwTable& tab) {
-      const int blocks = (int)std::min<uint32_t>(BLOCKS, tab.chunks);
+    auto go = [&](const GradTable& tab) {
+      // as many as give each the same number of chunks
+      const int64_t each = (tab.chunks + BLOCKS - 1) / BLOCKS;
+      const int blocks = (int)((tab.chunks + each - 1) / each);
       TORCH_CHECK(used + blocks <= partial.numel());
       CHECK_LAUNCH(launch_sumsq(cur_stream(), &tab, dtype, at + used, blocks));
       used += blocks;
     };
-    TableFiller<decltype(go)> fill(go);
-    for (const auto& g : grads)
-      if (g.numel() && adamw_dtype(g, "gradients") == dtype)
-        fill.add(nullptr, g.const_data_ptr(), nullptr, nullptr, nullptr,
-                 g.numel(), 0);
-    fill.flush();
+    GradTable tab;
+    tab.count = 0, tab.chunks = 0;
+    for (const auto& g : grads) {
+      if (!g.numel() || adamw_dtype(g, "gradients") != dtype) continue;
+      uint16_t tail;
+      const int64_t chunks = chunks_of(g.numel(), tail);
+      const int i = next_slot(tab, GRAD_TENSORS, chunks, go);
+      tab.g[i] = g.const_data_ptr(), tab.tail[i] = tail;
+    }
+    if (tab.count) go(tab);
   }
-  CHECK_LAUNCH(launch_norm_final(cur_stream(), at, used,
+  CHECK_LAUNCH(launch_norm_final(cur_stream(), at, (int)used,
                                  out.data_ptr<float>()));
   return out;
 }
@@ -460,7 +495,7 @@ c10::optional<torch::Tensor> adamw_step(
         fill.add(params[i].data_ptr(), grads[i].const_data_ptr(),
                  ms[i].data_ptr(), vs[i].data_ptr(),
                  eight ? scales[i].data_ptr() : nullptr, params[i].numel(),
-                 (uint32_t)i * 0x3C6EF372u);
+                 i);
     fill.flush();
   }
   return total_norm;

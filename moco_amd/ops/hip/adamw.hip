@@ -7,9 +7,10 @@
 //   m' = b1 m + (1 - b1) g        v' = b2 v + (1 - b2) g^2
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
-// Each operation is rounded by itself (no contraction into fma): a plain
-// elementwise program in 32 bits then computes the same values, and what is
-// rounded to 8 bits afterwards falls on the same codes.
+// Each operation is rounded by itself (no contraction into fma), as a plain
+// elementwise program in 32 bits does, so that what is rounded to 8 bits
+// afterwards falls on the same codes.  Root and reciprocal are the
+// hardware's, each off by an ulp at most.
 #include "common.h"
 #include "launchers.h"
 
@@ -23,16 +24,29 @@ constexpr int QBLOCK = 256;         // elements that share a pair of scales
 constexpr float TINY = 1e-30f;      // least block maximum a scale stands for
 constexpr float TOP_M = 448.f;      // largest e4m3 value
 constexpr float TOP_R = 1.9375f;    // largest value of a code of sqrt(v)
-static_assert(ADAMW_TENSORS == WAVE, "a wave looks up one tensor a lane");
+static_assert(sizeof(AdamwTable) + sizeof(AdamwScalars) + 16 <= 4096 &&
+                  sizeof(GradTable) + 8 <= 4096,
+              "kernel arguments");
 static_assert(CHUNK == THREADS * 16, "a thread handles 16 elements");
 
-// The tensor of chunk c: first[] ascends, so it is the last one whose first
-// chunk is not behind c.  One lane looks at each tensor.
-__device__ __forceinline__ int find_tensor(const uint32_t* first, int count,
-                                           uint32_t c) {
+// Where chunk c lies.  first[] ascends, so its tensor is the last one whose
+// first chunk is not behind c; a lane looks at one tensor in 64.
+struct Place {
+  int tensor;
+  int64_t at;  // first element
+  int left;    // elements, CHUNK at most
+};
+template <typename Table>
+__device__ __forceinline__ Place find_chunk(const Table& tab, uint32_t c) {
   const int lane = threadIdx.x % WAVE;
-  const bool before = lane < count && first[lane] <= c;
-  return __popcll(__ballot(before)) - 1;
+  int t = -1;
+  for (int b = 0; b < tab.count; b += WAVE) {
+    const int i = b + lane;
+    t += __popcll(__ballot(i < tab.count && tab.first[i] <= c));
+  }
+  const bool last = c + 1 == (t + 1 < tab.count ? tab.first[t + 1]
+                                                : tab.chunks);
+  return {t, (int64_t)(c - tab.first[t]) * CHUNK, last ? tab.tail[t] : CHUNK};
 }
 
 // V elements of type T as floats.  Tensors may be views that begin anywhere:
@@ -56,14 +70,14 @@ __device__ __forceinline__ void store_vec(T* p, const float (&in)[V]) {
 // the first `n` of them (n may be <= 0); zeros behind
 template <typename T, int V>
 __device__ __forceinline__ void load_part(const T* p, float (&out)[V],
-                                          int64_t n) {
+                                          int n) {
 #pragma unroll
   for (int i = 0; i < V; ++i) out[i] = i < n ? (float)p[i] : 0.f;
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void store_part(T* p, const float (&in)[V],
-                                           int64_t n) {
+                                           int n) {
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (i < n) p[i] = (T)in[i];
@@ -84,8 +98,8 @@ __device__ __forceinline__ void adamw_element(const AdamwScalars& h,
   g = g * coef;
   m = m * h.beta1 + g * h.one_minus_beta1;
   v = v * h.beta2 + (g * g) * h.one_minus_beta2;
-  r = __fsqrt_rn(v);
-  const float q = __fdiv_rn(m, r * h.inv_root_bc2 + h.eps);
+  r = __builtin_amdgcn_sqrtf(v);
+  const float q = m * __builtin_amdgcn_rcpf(r * h.inv_root_bc2 + h.eps);
   p = p * h.decay - q * h.step_size;
 }
 
@@ -96,13 +110,11 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(
     const AdamwTable tab, const AdamwScalars h, const float* norm) {
   constexpr int V = 16 / sizeof(T);
   constexpr int NV = CHUNK / (THREADS * V);
-  const int t = find_tensor(tab.first, tab.count, blockIdx.x);
-  const int64_t at = (int64_t)(blockIdx.x - tab.first[t]) * CHUNK;
+  const auto [t, at, left] = find_chunk(tab, blockIdx.x);
   T* p = (T*)tab.p[t] + at;
   const T* g = (const T*)tab.g[t] + at;
   float* m = (float*)tab.m[t] + at;
   float* v = (float*)tab.v[t] + at;
-  const int64_t left = tab.n[t] - at;
   const float coef = clip_coef(norm, h.max_norm);
   float gf[NV][V], pf[NV][V], mf[NV][V], vf[NV][V], r;
   const int i0 = threadIdx.x * V;
@@ -127,7 +139,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(
     }
   } else {
     for (int i = i0; i < left; i += THREADS * V) {
-      const int64_t n = left - i;
+      const int n = left - i;
       load_part(g + i, gf[0], n);
       load_part(p + i, pf[0], n);
       load_part(m + i, mf[0], n);
@@ -211,7 +223,7 @@ __device__ __forceinline__ uint2 pack_m(const float (&q)[8]) {
 }
 
 // bytes [0, n) of a code word, zeros behind
-__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int64_t n) {
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
   uint2 w = make_uint2(0, 0);
   if (n >= 8) {
     __builtin_memcpy(&w, p, 8);
@@ -225,7 +237,7 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int64_t n) {
   return w;
 }
 
-__device__ __forceinline__ void store_codes(uint8_t* p, uint2 w, int64_t n) {
+__device__ __forceinline__ void store_codes(uint8_t* p, uint2 w, int n) {
   if (n >= 8) {
     __builtin_memcpy(p, &w, 8);
   } else {
@@ -241,15 +253,13 @@ template <typename T>
 __global__ __launch_bounds__(THREADS) void adamw8_kernel(
     const AdamwTable tab, const AdamwScalars h, const float* norm,
     uint32_t seed) {
-  const int t = find_tensor(tab.first, tab.count, blockIdx.x);
-  const int64_t at = (int64_t)(blockIdx.x - tab.first[t]) * CHUNK;
+  const auto [t, at, left] = find_chunk(tab, blockIdx.x);
   T* p = (T*)tab.p[t] + at;
   const T* g = (const T*)tab.g[t] + at;
   uint8_t* m = (uint8_t*)tab.m[t] + at;
   uint8_t* v = (uint8_t*)tab.v[t] + at;
   const int b = threadIdx.x / 16, l = threadIdx.x % 16;
   float2* scale = (float2*)tab.s[t] + at / QBLOCK + b;
-  const int64_t left = tab.n[t] - at;
   const bool full = left >= CHUNK;
   const float coef = clip_coef(norm, h.max_norm);
   const int i0 = b * QBLOCK + l * 8;
@@ -286,19 +296,22 @@ __global__ __launch_bounds__(THREADS) void adamw8_kernel(
       top_r = max(top_r, __float_as_uint(rf[j][k]) & 0x7FFFFFFFu);
     }
   }
-  const float sm = __uint_as_float(max16(top_m)) * (float)(1.0 / 448.0);
-  const float sr = __uint_as_float(max16(top_r)) * (float)(1.0 / 1.9375);
-  const float im = __frcp_rn(sm), ir = __frcp_rn(sr);
-  const uint32_t key = seed + tab.key[t] + (uint32_t)at;
+  float sm = __uint_as_float(max16(top_m)) * (float)(1.0 / 448.0);
+  float sr = __uint_as_float(max16(top_r)) * (float)(1.0 / 1.9375);
+  // an infinity in the block: all of it becomes a NaN, whatever the codes
+  if (!(sm < INFINITY)) sm = NAN;
+  if (!(sr < INFINITY)) sr = NAN;
+  const float im = 1.f / sm, ir = 1.f / sr;
+  const uint32_t key =
+      seed + (tab.list_base + tab.number[t]) * 0x3C6EF372u + (uint32_t)at;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int i = i0 + j * 128;
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      // clamped with comparisons: a NaN stays a NaN
-      const float q = mf[j][k] * im;
-      mf[j][k] = q > TOP_M ? TOP_M : q < -TOP_M ? -TOP_M : q;
+      // (where this is a NaN so is the scale: the code says nothing)
+      mf[j][k] = __builtin_amdgcn_fmed3f(mf[j][k] * im, -TOP_M, TOP_M);
       w[k / 4] |= encode_root(rf[j][k] * ir, dither19(key + i + k))
                   << (8 * (k % 4));
     }
@@ -320,13 +333,11 @@ __global__ __launch_bounds__(THREADS) void adamw8_kernel(
 template <typename T>
 __global__ __launch_bounds__(THREADS) void adamw8_values_kernel(
     const AdamwTable tab) {
-  const int t = find_tensor(tab.first, tab.count, blockIdx.x);
-  const int64_t at = (int64_t)(blockIdx.x - tab.first[t]) * CHUNK;
-  const int64_t left = tab.n[t] - at;
+  const auto [t, at, left] = find_chunk(tab, blockIdx.x);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int i = (j * THREADS + threadIdx.x) * 8;
-    const int64_t n = left - i;
+    const int n = left - i;
     if (n <= 0) break;
     const uint2 mc = load_codes((const uint8_t*)tab.m[t] + at + i, n);
     const uint2 vc = load_codes((const uint8_t*)tab.v[t] + at + i, n);
@@ -357,21 +368,24 @@ __global__ __launch_bounds__(THREADS) void adamw8_values_kernel(
 // 4 (2) bytes an element.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void sumsq_kernel(
-    const AdamwTable tab, double* __restrict__ partial) {
+    const GradTable tab, double* __restrict__ partial) {
   constexpr int V = 16 / sizeof(T);
+  constexpr int NV = CHUNK / (THREADS * V);
   double acc = 0.0;
   for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    const int t = find_tensor(tab.first, tab.count, c);
-    const int64_t at = (int64_t)(c - tab.first[t]) * CHUNK;
-    const T* g = (const T*)tab.g[t] + at;
-    const int64_t left = tab.n[t] - at;
-    float gf[V];
-    for (int i = threadIdx.x * V; i < CHUNK && i < left; i += THREADS * V) {
-      if (left - i >= V) load_vec(g + i, gf);
-      else load_part(g + i, gf, left - i);
+    const auto [t, at, left] = find_chunk(tab, c);
+    const T* g = (const T*)tab.g[t] + at + threadIdx.x * V;
+    const int n = left - threadIdx.x * V;
+    float gf[NV][V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc += (double)gf[k] * (double)gf[k];
+    for (int j = 0; j < NV; ++j) {
+      if (left == CHUNK) load_vec(g + j * THREADS * V, gf[j]);
+      else load_part(g + j * THREADS * V, gf[j], n - j * THREADS * V);
     }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc += (double)gf[j][k] * (double)gf[j][k];
   }
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, WAVE);
   __shared__ double part[THREADS / WAVE];
@@ -384,6 +398,7 @@ __global__ __launch_bounds__(THREADS) void sumsq_kernel(
 __global__ __launch_bounds__(THREADS) void norm_final_kernel(
     const double* __restrict__ partial, int n, float* __restrict__ out) {
   double acc = 0.0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < n; i += THREADS) acc += partial[i];
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, WAVE);
   __shared__ double part[THREADS / WAVE];
@@ -411,7 +426,7 @@ void go_values(hipStream_t s, const AdamwTable& tab) {
 }
 
 template <typename T>
-void go_sumsq(hipStream_t s, const AdamwTable& tab, double* partial,
+void go_sumsq(hipStream_t s, const GradTable& tab, double* partial,
               int blocks) {
   sumsq_kernel<T><<<dim3(blocks), THREADS, 0, s>>>(tab, partial);
 }
@@ -452,7 +467,7 @@ extern "C" int launch_adamw8_values(void* stream, const AdamwTable* tab,
   return 0;
 }
 
-extern "C" int launch_sumsq(void* stream, const AdamwTable* tab, int dtype,
+extern "C" int launch_sumsq(void* stream, const GradTable* tab, int dtype,
                             double* partial, int blocks) {
   if (tab->chunks == 0 || blocks == 0) return 0;
   BY_DTYPE(dtype, go_sumsq, (hipStream_t)stream, *tab, partial, blocks)

@@ -58,12 +58,13 @@ int launch_ema_flat(void* stream, float* dst, const float* src, int64_t n,
 
 // ---- adamw.hip ------------------------------------------------------------
 // A table of up to ADAMW_TENSORS tensors of one dtype, passed by value in
-// the kernel's arguments.  Tensor i has n[i] elements, at p (weights), g
+// the kernel's arguments (which hold 4 KB).  Tensor i is at p (weights), g
 // (gradients), m and v (moments, fp32 or 8-bit codes) and s (fp32 pairs of
-// scales, one per 256 elements; 8-bit only), and takes the chunks of
-// ADAMW_CHUNK elements from first[i] on; key[i] is its number in the
-// caller's list, spread over 32 bits.  dtype: 0 fp32, 1 bf16, 2 fp16.
-#define ADAMW_TENSORS 64
+// scales, one per 256 elements; 8-bit only).  It takes the chunks of
+// ADAMW_CHUNK elements from first[i] on, of which the last has tail[i]; its
+// number in the caller's list is list_base + number[i].  dtype: 0 fp32,
+// 1 bf16, 2 fp16.
+#define ADAMW_TENSORS 82
 #define ADAMW_CHUNK 4096
 struct AdamwTable {
   void* p[ADAMW_TENSORS];
@@ -71,9 +72,18 @@ struct AdamwTable {
   void* m[ADAMW_TENSORS];
   void* v[ADAMW_TENSORS];
   void* s[ADAMW_TENSORS];
-  int64_t n[ADAMW_TENSORS];
   uint32_t first[ADAMW_TENSORS];
-  uint32_t key[ADAMW_TENSORS];
+  uint16_t tail[ADAMW_TENSORS];
+  uint16_t number[ADAMW_TENSORS];
+  uint32_t list_base, chunks;
+  int count;
+};
+// the same for gradients alone
+#define GRAD_TENSORS 256
+struct GradTable {
+  const void* g[GRAD_TENSORS];
+  uint32_t first[GRAD_TENSORS];
+  uint16_t tail[GRAD_TENSORS];
   uint32_t chunks;
   int count;
 };
@@ -89,7 +99,7 @@ int launch_adamw8(void* stream, const AdamwTable* tab, const AdamwScalars* h,
 // decoded moments of the codes m, v, s into p (m) and g (v), of type dtype
 int launch_adamw8_values(void* stream, const AdamwTable* tab, int dtype);
 // partial[blocks]: sums of squares of the table's g
-int launch_sumsq(void* stream, const AdamwTable* tab, int dtype,
+int launch_sumsq(void* stream, const GradTable* tab, int dtype,
                  double* partial, int blocks);
 // out = sqrt(sum of partial[0..n))
 int launch_norm_final(void* stream, const double* partial, int n, float* out);

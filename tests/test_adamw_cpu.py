@@ -126,9 +126,9 @@ def test_grad_norm_mixes_types_and_counts_expanded_elements():
 def test_nonfinite_gradients():
     """A NaN reaches the weight it belongs to, and with 8-bit moments its
     block's scale; under a clip it reaches all."""
-    for eight in (False, True):
+    for eight, value in ((False, "nan"), (True, "nan"), (True, "inf")):
         state = make([(600,)], eight=eight)
-        state[1][0][300] = float("nan")
+        state[1][0][300] = float(value)
         (adamw8bit_ if eight else adamw_)(*state, step=1, lr=0.1)
         bad = torch.isnan(state[0][0])
         assert bad.sum() == 1 and bad[300]
