@@ -129,10 +129,12 @@ __device__ __forceinline__ void load_vec(const void* p, bool f32,
   }
 }
 
-// Sum over a wave, the same in all lanes: inside rows of 16 lanes by DPP, the
-// four rows through scalar registers.  (Six ds_bpermute steps take some 400
-// cycles of latency, twice or more a row.)
-__device__ __forceinline__ float wave_sum(float v) {
+// Sum over the N lanes (8 to 64) that share a row, the same in all of them:
+// inside rows of 16 lanes by DPP, a wave's four through scalar registers.
+// (Six ds_bpermute steps take some 400 cycles of latency, twice or more a
+// row.)
+template <int N>
+__device__ __forceinline__ float lane_sum(float v) {
   auto dpp = [](float x, auto ctrl) {
     return __int_as_float(__builtin_amdgcn_update_dpp(
         0, __float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, true));
@@ -140,7 +142,10 @@ __device__ __forceinline__ float wave_sum(float v) {
   v += dpp(v, std::integral_constant<int, 0xB1>());   // lane ^ 1
   v += dpp(v, std::integral_constant<int, 0x4E>());   // lane ^ 2
   v += dpp(v, std::integral_constant<int, 0x141>());  // half row mirrored
-  v += dpp(v, std::integral_constant<int, 0x140>());  // row mirrored
+  if constexpr (N >= 16)
+    v += dpp(v, std::integral_constant<int, 0x140>());  // row mirrored
+  if constexpr (N == 32) v += __shfl_xor(v, 16, WAVE);
+  if constexpr (N < WAVE) return v;
   const int b = __float_as_int(v);
   return (__int_as_float(__builtin_amdgcn_readlane(b, 0)) +
           __int_as_float(__builtin_amdgcn_readlane(b, 16))) +
@@ -148,16 +153,24 @@ __device__ __forceinline__ float wave_sum(float v) {
           __int_as_float(__builtin_amdgcn_readlane(b, 48)));
 }
 
+// the group of NT threads that this one belongs to: where that is whole
+// waves, in a scalar register, and so is what is made of it
+template <int NT>
+__device__ __forceinline__ int group_of() {
+  return NT < WAVE ? threadIdx.x / NT
+                   : __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+}
+
 // sums of M values over the NT threads of a row, in a fixed order
 template <int NT, int M>
 struct RowSum {
-  static constexpr int WAVES = NT / WAVE;  // of this row
+  static constexpr int WAVES = NT / WAVE;  // of this row (0: part of one)
   // two slots in turn: one barrier a reduction
   float slot[2][M][WAVES > 1 ? WAVES : 1];
 
   __device__ __forceinline__ void operator()(float (&v)[M], int turn) {
 #pragma unroll
-    for (int j = 0; j < M; ++j) v[j] = wave_sum(v[j]);
+    for (int j = 0; j < M; ++j) v[j] = lane_sum<(NT < WAVE ? NT : WAVE)>(v[j]);
     if constexpr (WAVES > 1) {
       const int wave = threadIdx.x / WAVE % WAVES;
       if (threadIdx.x % WAVE == 0)
@@ -269,7 +282,7 @@ __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_fwd_kernel(
   constexpr int GROUPS = NT < BLOCK ? BLOCK / NT : 1;
   constexpr bool KEEP = K == 1;
   __shared__ RowSum<NT, 1> sums[GROUPS];
-  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const int group = group_of<NT>();
   const int t = threadIdx.x % NT;
   RowSum<NT, 1>& sum = sums[group];
   int turn = 0;
@@ -376,7 +389,7 @@ constexpr int VECS = 5;
 // read from LDS (K = 1), where a workgroup puts them once.
 template <typename TX, typename TH, int NT, int K, int V, bool LAYER>
 __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT,
-                             LAYER && NT < 1024 ? 3 : 4) void
+                             NT < WAVE || (LAYER && NT < 1024) ? 3 : 4) void
 norm_bwd_kernel(const NormArgs a, const NormGrads o) {
   constexpr int GROUPS = NT < BLOCK ? BLOCK / NT : 1;
   constexpr bool KEEP = K == 1;
@@ -389,7 +402,7 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
   __shared__ float kept[KEEP ? KEPT : 1][KEEP ? Q : 1][KEEP ? NT : 1][W];
   __shared__ float across[GROUPS > 1 ? GROUPS : 1]
                          [GROUPS > 1 ? NT * K * V : 1];
-  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const int group = group_of<NT>();
   const int t = threadIdx.x % NT;
   RowSum<NT, 2>& sum2 = sums2[group];
   RowSum<NT, 3>& sum3 = sums3[group];
@@ -466,17 +479,17 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
       row_slope[0] = (float)((const TH*)a.gate)[row * a.ld_g];
       activate(a.act, row_slope, row_act);
     }
-    float d[K][V], act[K][V], slope[K][V];
+    float d[K][V], act[V], slope[V];
+    auto gate = [&](int k) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) act[k][i] = row_act[0], slope[k][i] = 1.f;
+      for (int i = 0; i < V; ++i) act[i] = row_act[0], slope[i] = 1.f;
       if (full) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) slope[k][i] = g[k][i];
-        activate(a.act, slope[k], act[k]);
+        for (int i = 0; i < V; ++i) slope[i] = g[k][i];
+        activate(a.act, slope, act);
       }
-    }
+    };
+    if (K == 1) gate(0);
     auto hat_h = [&](int k, int i) {
       return (LAYER ? h[k][i] - mean_h : h[k][i]) * rstd_h;
     };
@@ -486,6 +499,7 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float v[V];
+        if (K > 1) gate(k);
         if (a.h != nullptr) {
           vec(0, k, v);
 #pragma unroll
@@ -498,7 +512,7 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
           vec(1, k, v);
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            d[k][i] = x[k][i] + v[i] * act[k][i] * d[k][i];
+            d[k][i] = x[k][i] + v[i] * act[i] * d[k][i];
         } else {
 #pragma unroll
           for (int i = 0; i < V; ++i) d[k][i] = x[k][i];
@@ -544,6 +558,7 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float w[V], s[V], nf[V];
+      if (K > 1) gate(k);
       vec(0, k, w);
 #pragma unroll
       for (int i = 0; i < V; ++i) nf[i] = hat_h(k, i) * w[i];
@@ -557,9 +572,9 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float dsn = d[k][i] * nf[i];
-        acc[4][k][i] += dsn * act[k][i];
-        slope[k][i] *= dsn * s[i];
-        const float dn = d[k][i] * (s[i] * act[k][i]);
+        acc[4][k][i] += dsn * act[i];
+        slope[i] *= dsn * s[i];
+        const float dn = d[k][i] * (s[i] * act[i]);
         acc[0][k][i] += dn * hat_h(k, i);
         if (LAYER) acc[1][k][i] += dn;
         d[k][i] = dn * w[i];  // t1 from here on
@@ -568,11 +583,11 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
         if (LAYER) q[1] += t1;
       }
       if (full && o.d_gate != nullptr && in)
-        store_f<TH>(o.d_gate, row * a.width, c[k], slope[k]);
+        store_f<TH>(o.d_gate, row * a.width, c[k], slope);
       if (per_row) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          q[2] += i >= c[k].skip ? slope[k][i] : 0.f;
+          q[2] += i >= c[k].skip ? slope[i] : 0.f;
       }
     }
     if (a.post != NORM_NONE || per_row) sum3(q, turn);
@@ -616,22 +631,31 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
 }
 
 // out[c] = sum over blocks of partial[b][c], for up to VECS vectors; one
-// workgroup adds 64 columns, 16 parts of the blocks side by side
+// workgroup adds 32 columns (a line of memory), 32 parts of the blocks side
+// by side with 8 loads each on their way (16 parts and one load at a time
+// took 10 us for 512 blocks of any width)
 __global__ __launch_bounds__(1024) void norm_columns_kernel(
     const NormColumns v, int blocks, int width) {
-  const float* p = v.partial[blockIdx.y];
-  const int c = blockIdx.x * 64 + threadIdx.x % 64;
-  const int part = threadIdx.x / 64;
+  const int lane = threadIdx.x % 32, part = threadIdx.x / 32;
+  const int c = min((int)blockIdx.x * 32 + lane, width - 1);
+  const float* p = v.partial[blockIdx.y] + c;
   float s = 0.f;
-  if (c < width)
-    for (int b = part; b < blocks; b += 16) s += p[(int64_t)b * width + c];
-  __shared__ float lds[16][64];
-  lds[part][threadIdx.x % 64] = s;
+  int b = part;
+  for (; b + 7 * 32 < blocks; b += 8 * 32) {
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = p[(int64_t)(b + j * 32) * width];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += f[j];
+  }
+  for (; b < blocks; b += 32) s += p[(int64_t)b * width];
+  __shared__ float lds[32][33];
+  lds[part][lane] = s;
   __syncthreads();
-  if (part != 0 || c >= width) return;
+  if (part != 0 || (int)blockIdx.x * 32 + lane >= width) return;
   s = 0.f;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) s += lds[j][threadIdx.x];
+  for (int j = 0; j < 32; ++j) s += lds[j][lane];
   void* out = v.out[blockIdx.y];
   switch (v.dtype[blockIdx.y]) {
     case 0: ((float*)out)[c] = s; break;
@@ -666,7 +690,10 @@ void go(hipStream_t s, const NormArgs& a, const NormGrads* o, int blocks) {
 template <typename TX, typename TH>
 int go_width(hipStream_t s, const NormArgs& a, const NormGrads* o,
              int blocks) {
-  if (a.width < 8) go<TX, TH, 64, 1, 1>(s, a, o, blocks);
+  if (a.width < 8) go<TX, TH, 8, 1, 1>(s, a, o, blocks);
+  else if (a.width <= 64) go<TX, TH, 8, 1, 8>(s, a, o, blocks);
+  else if (a.width <= 128) go<TX, TH, 16, 1, 8>(s, a, o, blocks);
+  else if (a.width <= 256) go<TX, TH, 32, 1, 8>(s, a, o, blocks);
   else if (a.width <= 512) go<TX, TH, 64, 1, 8>(s, a, o, blocks);
   else if (a.width <= 1024) go<TX, TH, 128, 1, 8>(s, a, o, blocks);
   else if (a.width <= 2048) go<TX, TH, 256, 1, 8>(s, a, o, blocks);
@@ -698,7 +725,12 @@ extern "C" int launch_norm_fwd(void* stream, const NormArgs* a) {
 }
 
 extern "C" int norm_bwd_blocks(int64_t rows, int64_t width) {
-  const int64_t groups = width <= 512 ? 4 : width <= 1024 ? 2 : 1;
+  const int64_t groups = width <= 64    ? 32
+                         : width <= 128 ? 16
+                         : width <= 256 ? 8
+                         : width <= 512 ? 4
+                         : width <= 1024 ? 2
+                                         : 1;
   const int64_t most = (rows + groups - 1) / groups;
   return (int)(most < 512 ? most : 512);
 }
@@ -712,7 +744,7 @@ extern "C" int launch_norm_bwd(void* stream, const NormArgs* a,
 extern "C" int launch_norm_columns(void* stream, const NormColumns* v,
                                    int vecs, int blocks, int64_t width) {
   if (vecs == 0 || width == 0) return 0;
-  norm_columns_kernel<<<dim3((unsigned)((width + 63) / 64), vecs), 1024, 0,
+  norm_columns_kernel<<<dim3((unsigned)((width + 31) / 32), vecs), 1024, 0,
                         (hipStream_t)stream>>>(*v, blocks, (int)width);
   HIP_CHECK_LAST();
   return 0;

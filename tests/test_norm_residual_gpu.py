@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 
 # one row to several per workgroup; widths around a vector of 8, and of each
 # number of threads and registers per row
-SIZES = [(1, 1), (1, 2048), (5, 7), (3, 64), (130, 65), (9, 512), (6, 513),
+SIZES = [(1, 1), (1, 2048), (5, 7), (70, 8), (3, 9), (3, 64), (130, 65),
+         (77, 128), (50, 129), (40, 256), (9, 257), (9, 512), (6, 513),
          (600, 200), (7, 1000), (5, 1024), (4, 1025), (3, 2048), (520, 1030),
          (3, 2056), (2, 4095), (5, 4096), (2, 4100), (2, 8192), (2, 8195),
          (3, 16383), (2, 16384)]
