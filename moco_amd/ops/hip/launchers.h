@@ -137,7 +137,7 @@ struct NormColumns {
   int dtype[5];
 };
 int launch_norm_fwd(void* stream, const NormArgs* a);
-int norm_bwd_blocks(int64_t rows, int64_t width);
+int norm_bwd_blocks(const NormArgs* a);
 int launch_norm_bwd(void* stream, const NormArgs* a, const NormGrads* o,
                     int blocks);
 int launch_norm_columns(void* stream, const NormColumns* v, int vecs,
