@@ -223,8 +223,7 @@ def _adamw(params, grads, ms, vs, scales, step, lr, betas, eps, weight_decay,
     params, grads = list(params), list(grads)
     if use_hip(*params[:1]):
         return ext().adamw_step(
-            params, grads, ms, vs, [] if scales is None else scales,
-            scales is not None, int(step), lr, betas[0], betas[1], eps,
+            params, grads, ms, vs, scales, int(step), lr, betas[0], betas[1], eps,
             weight_decay, max_norm, total_norm, seed & 0xFFFFFFFF)
     _check_lists(params, grads, ms, vs, scales)
     if not params:
@@ -454,6 +453,9 @@ class FusedAdamW(torch.optim.Optimizer):
         """Also takes the state of torch.optim.AdamW.  The moments keep their
         own types (the base class casts them to the parameter's) and follow
         their parameter's memory format."""
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("amsgrad and maximize are not supported")
         super().load_state_dict(state_dict)
         for group in self.param_groups:
             group.setdefault("state_bits", 32)

@@ -9,6 +9,7 @@
 
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <array>
@@ -251,6 +252,29 @@ void ema_flat(torch::Tensor dst, torch::Tensor src, double m) {
 
 using TensorList = std::vector<torch::Tensor>;
 
+// The tensors of a Python list, borrowed: its items hold them during the
+// call (owning copies of 800 tensors cost as much time as all checks).
+struct Refs {
+  std::vector<const torch::Tensor*> t;
+  py::object hold;
+  Refs() = default;
+  explicit Refs(const py::object& list)
+      : hold(py::reinterpret_steal<py::object>(PySequence_Fast(
+            list.ptr(), "a list of tensors is expected"))) {
+    if (!hold) throw py::error_already_set();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(hold.ptr());
+    t.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* x = PySequence_Fast_GET_ITEM(hold.ptr(), i);
+      TORCH_CHECK_TYPE(THPVariable_Check(x), "a list of tensors is expected");
+      t.push_back(&THPVariable_Unpack(x));
+    }
+  }
+  size_t size() const { return t.size(); }
+  bool empty() const { return t.empty(); }
+  const torch::Tensor& operator[](size_t i) const { return *t[i]; }
+};
+
 int adamw_dtype(const torch::Tensor& t, const char* what) {
   switch (t.scalar_type()) {
     case torch::kFloat32: return 0;
@@ -281,6 +305,7 @@ struct Range {
 };
 
 void add_range(std::vector<Range>& r, const torch::Tensor& t, bool write) {
+  if (t.numel() == 0) return;
   const uintptr_t a = (uintptr_t)t.const_data_ptr();
   r.push_back({a, a + t.numel() * t.element_size(), write});
 }
@@ -349,14 +374,14 @@ struct TableFiller {
 };
 
 // 2-norm over all elements of a list; every tensor dense, on one device
-torch::Tensor grad_norm_checked(const TensorList& grads) {
+torch::Tensor grad_norm_checked(const Refs& grads) {
   auto opts = grads[0].options().dtype(torch::kFloat32).layout(torch::kStrided);
   auto out = torch::empty({}, opts);
   // workgroups of a launch at most: 8 per CU, which fill it with loads
   constexpr int64_t BLOCKS = 2048;
   // a launch takes GRAD_TENSORS tensors of one dtype or MOST_CHUNKS chunks
   int64_t launches = (int64_t)grads.size() / GRAD_TENSORS + 3, elements = 0;
-  for (const auto& g : grads) elements += g.numel();
+  for (const auto* g : grads.t) elements += g->numel();
   launches += 2 * (elements / ADAMW_CHUNK + (int64_t)grads.size()) /
               MOST_CHUNKS;
   auto partial = torch::empty({launches * BLOCKS},
@@ -374,12 +399,12 @@ torch::Tensor grad_norm_checked(const TensorList& grads) {
     };
     GradTable tab;
     tab.count = 0, tab.chunks = 0;
-    for (const auto& g : grads) {
-      if (!g.numel() || adamw_dtype(g, "gradients") != dtype) continue;
+    for (const auto* g : grads.t) {
+      if (!g->numel() || adamw_dtype(*g, "gradients") != dtype) continue;
       uint16_t tail;
-      const int64_t chunks = chunks_of(g.numel(), tail);
+      const int64_t chunks = chunks_of(g->numel(), tail);
       const int i = next_slot(tab, GRAD_TENSORS, chunks, go);
-      tab.g[i] = g.const_data_ptr(), tab.tail[i] = tail;
+      tab.g[i] = g->const_data_ptr(), tab.tail[i] = tail;
     }
     if (tab.count) go(tab);
   }
@@ -388,37 +413,47 @@ torch::Tensor grad_norm_checked(const TensorList& grads) {
   return out;
 }
 
-torch::Tensor grad_norm(const TensorList& grads) {
+torch::Tensor grad_norm(const py::object& list) {
+  Refs grads(list);
   TORCH_CHECK_VALUE(!grads.empty(), "grad_norm needs at least one tensor");
-  at::cuda::CUDAGuard guard(grads[0].device());
-  TensorList dense;
-  for (const auto& g : grads) {
-    TORCH_CHECK_VALUE(g.device() == grads[0].device() && g.is_cuda(),
+  const auto device = grads[0].device();
+  TORCH_CHECK_VALUE(device.is_cuda(), "gradients must be on one device");
+  at::cuda::CUDAGuard guard(device);
+  TensorList copies;
+  copies.reserve(grads.size());  // their addresses are taken
+  for (auto& g : grads.t) {
+    TORCH_CHECK_VALUE(g->device() == device,
                       "gradients must be on one device");
-    TORCH_CHECK_VALUE(g.layout() == torch::kStrided,
+    TORCH_CHECK_VALUE(g->layout() == torch::kStrided,
                       "sparse gradients are not supported");
-    adamw_dtype(g, "gradients");
+    adamw_dtype(*g, "gradients");
     // an expanded or gapped view is laid out first: each element counts once
     // per place that it has in the tensor
-    dense.push_back(g.is_non_overlapping_and_dense() ? g : g.contiguous());
+    if (g->is_non_overlapping_and_dense()) continue;
+    copies.push_back(g->contiguous());
+    g = &copies.back();
   }
-  return grad_norm_checked(dense);
+  return grad_norm_checked(grads);
 }
 
 // One AdamW step (8-bit moments where `scales` is not empty).  Returns the
 // gradient norm that the clip went by, if there was one.
 c10::optional<torch::Tensor> adamw_step(
-    const TensorList& params, const TensorList& grads, const TensorList& ms,
-    const TensorList& vs, const TensorList& scales, bool eight, int64_t step,
+    const py::object& params_, const py::object& grads_, const py::object& ms_,
+    const py::object& vs_, const py::object& scales_, int64_t step,
     double lr, double beta1, double beta2, double eps, double weight_decay,
     c10::optional<double> max_norm, c10::optional<torch::Tensor> total_norm,
     int64_t seed) {
+  const bool eight = !scales_.is_none();
+  const Refs params(params_), grads(grads_), ms(ms_), vs(vs_);
+  const Refs scales = eight ? Refs(scales_) : Refs();
   const size_t n = params.size();
   TORCH_CHECK_VALUE(grads.size() == n && ms.size() == n && vs.size() == n &&
                         scales.size() == (eight ? n : 0),
                     "the lists of tensors differ in length");
   if (n == 0) return total_norm;
   const auto device = params[0].device();
+  TORCH_CHECK_VALUE(device.is_cuda(), "all tensors must be on one device");
   at::cuda::CUDAGuard guard(device);
   std::vector<Range> ranges;
   ranges.reserve(5 * n);
@@ -499,18 +534,24 @@ c10::optional<torch::Tensor> adamw_step(
                  i);
     fill.flush();
   }
+  // autograd's count of writes: a graph that saved a weight notices
+  for (const Refs* list : {&params, &ms, &vs, &scales})
+    for (const auto* t : list->t) t->unsafeGetTensorImpl()->bump_version();
   return total_norm;
 }
 
 // decoded moments of 8-bit codes
-std::vector<TensorList> adamw8bit_values(const TensorList& ms,
-                                         const TensorList& vs,
-                                         const TensorList& scales,
-                                         torch::ScalarType dtype) {
+std::pair<TensorList, TensorList> adamw8bit_values(const py::object& ms_,
+                                                   const py::object& vs_,
+                                                   const py::object& scales_,
+                                                   const py::object& dtype_) {
+  const Refs ms(ms_), vs(vs_), scales(scales_);
+  const auto dtype = torch::python::detail::py_object_to_dtype(dtype_);
   TORCH_CHECK_VALUE(vs.size() == ms.size() && scales.size() == ms.size(),
                     "the lists of tensors differ in length");
-  std::vector<TensorList> out(2);
+  std::pair<TensorList, TensorList> out;
   if (ms.empty()) return out;
+  TORCH_CHECK_VALUE(ms[0].is_cuda(), "all tensors must be on one device");
   at::cuda::CUDAGuard guard(ms[0].device());
   int kind = 0;
   auto go = [&](const AdamwTable& tab) {
@@ -543,8 +584,8 @@ std::vector<TensorList> adamw8bit_values(const TensorList& ms,
     if (m.numel())
       fill.add(om.data_ptr(), ov.data_ptr(), m.data_ptr(), v.data_ptr(),
                s.data_ptr(), m.numel(), 0);
-    out[0].push_back(om);
-    out[1].push_back(ov);
+    out.first.push_back(om);
+    out.second.push_back(ov);
   }
   fill.flush();
   return out;
@@ -1339,11 +1380,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("grad_norm", &grad_norm);
   mod.def("norm_residual", &norm_residual);
   mod.def("adamw_step", &adamw_step);
-  mod.def("adamw8bit_values", [](const TensorList& m, const TensorList& v,
-                                 const TensorList& s, py::object dtype) {
-    return adamw8bit_values(
-        m, v, s, torch::python::detail::py_object_to_dtype(dtype));
-  });
+  mod.def("adamw8bit_values", &adamw8bit_values);
   mod.def("two_crop_augment", &two_crop_augment);
   mod.def("bn_fwd_train", &bn_fwd_train);
   mod.def("bn_fwd_eval", &bn_fwd_eval);

@@ -300,6 +300,22 @@ def test_one_gradient_for_two_weights_is_allowed():
     assert torch.equal(ms[0], ms[1])
 
 
+def test_writes_are_counted():
+    """A graph that saved a weight notices that it has changed."""
+    for eight in (False, True):
+        state = make([(300,)], eight=eight)
+        was = [x[0]._version for x in state]
+        (adamw8bit_ if eight else adamw_)(*state, step=1, lr=0.1)
+        assert [x[0]._version > w for x, w in zip(state, was)] == \
+            [True, False] + [True] * (len(state) - 2)
+
+
+def test_empty_view_inside_another_tensor():
+    ps, gs, ms, vs = make([(300,), (0,)])
+    ps[1] = ps[0][7:7]
+    adamw_(ps, gs, ms, vs, step=1, lr=0.1)
+
+
 def test_empty_lists():
     assert adamw_([], [], [], [], step=1, lr=0.1) is None
     assert adamw8bit_([], [], [], [], [], step=1, lr=0.1) is None
@@ -431,6 +447,10 @@ def test_loaded_state_follows_the_memory_format(bits):
 
 
 def test_optimizer_refusals():
+    p = params()
+    other = torch.optim.AdamW(p, lr=0.1, amsgrad=True)
+    with pytest.raises(ValueError):
+        FusedAdamW(p).load_state_dict(other.state_dict())
     with pytest.raises(ValueError):
         FusedAdamW(params(), state_bits=4)
     with pytest.raises(ValueError):

@@ -302,6 +302,24 @@ def test_refusals_gpu():
         grad_norm([torch.zeros(3, device="cuda", dtype=torch.float64)])
 
 
+def test_writes_are_counted_and_empty_views_allowed():
+    from moco_amd.ops import adamw8bit_, adamw_
+    for eight in (False, True):
+        st = make([(300,), (0,)], torch.float32, eight)
+        st[0][1] = st[0][0][7:7]
+        gs = grads_for(st[0], 0)
+        was = [st[0][0]._version, gs[0]._version] + [
+            x[0]._version for x in st[1:]]
+        (adamw8bit_ if eight else adamw_)(st[0], gs, *st[1:], step=1, lr=0.1)
+        now = [st[0][0]._version, gs[0]._version] + [
+            x[0]._version for x in st[1:]]
+        assert [a > b for a, b in zip(now, was)] == \
+            [True, False] + [True] * (len(st) - 1)
+        with pytest.raises(TypeError):
+            (adamw8bit_ if eight else adamw_)([st[0][0]], [3], *st[1:],
+                                              step=1, lr=0.1)
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_optimizer_gpu(bits):
     """A model in channels_last with bf16 and fp32 weights; the CPU's plain
