@@ -204,7 +204,7 @@ def grad_norm(grads: Tensors) -> torch.Tensor:
     if not grads:
         raise ValueError("grad_norm needs at least one tensor")
     if use_hip(*grads[:1]):
-        return ext().grad_norm(grads)
+        return ext().grad_norm(grads, False)
     for g in grads:
         if g.layout != torch.strided:
             raise ValueError("sparse gradients are not supported")
@@ -437,7 +437,10 @@ class FusedAdamW(torch.optim.Optimizer):
                 every_grad.append(g)
         norm = None
         if self.max_grad_norm is not None and every_grad:
-            norm = self.last_grad_norm = grad_norm(every_grad)
+            # (on the GPU: read through the caches, for the step's sake)
+            norm = self.last_grad_norm = \
+                ext().grad_norm(every_grad, True) \
+                if use_hip(every_grad[0]) else grad_norm(every_grad)
         for n, ((gi, count, eight), lists) in enumerate(buckets.items()):
             group = self.param_groups[gi]
             # each bucket's list counts from 0: a hash of its own

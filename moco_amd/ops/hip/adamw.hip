@@ -49,22 +49,41 @@ __device__ __forceinline__ Place find_chunk(const Table& tab, uint32_t c) {
   return {t, (int64_t)(c - tab.first[t]) * CHUNK, last ? tab.tail[t] : CHUNK};
 }
 
-// V elements of type T as floats.  Tensors may be views that begin anywhere:
-// only the element's own alignment is assumed.
+// V elements of type T as they lie in memory.  Tensors may be views that
+// begin anywhere: only the element's own alignment is assumed.  ONCE: past
+// the caches, for what will not be there when it is next used.
+typedef uint32_t word4 __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&out)[V]) {
-  T raw[V];
-  __builtin_memcpy(raw, p, sizeof(raw));
+struct Raw {
+  static constexpr int W = sizeof(T) * V / 16;
+  word4 w[W];
+  template <bool ONCE>
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = (float)raw[i];
-}
+    for (int i = 0; i < W; ++i)
+      w[i] = ONCE ? __builtin_nontemporal_load((const word4*)p + i)
+                  : *((const word4*)p + i);
+  }
+  __device__ __forceinline__ void floats(float (&out)[V]) const {
+    T t[V];
+    __builtin_memcpy(t, w, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = (float)t[i];
+  }
+};
 
-template <typename T, int V>
+template <bool ONCE, typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&in)[V]) {
-  T raw[V];
+  T t[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) raw[i] = (T)in[i];  // to nearest even
-  __builtin_memcpy(p, raw, sizeof(raw));
+  for (int i = 0; i < V; ++i) t[i] = (T)in[i];  // to nearest even
+  word4 w[sizeof(t) / 16];
+  __builtin_memcpy(w, t, sizeof(t));
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(t) / 16; ++i) {
+    if (ONCE) __builtin_nontemporal_store(w[i], (word4*)p + i);
+    else *((word4*)p + i) = w[i];
+  }
 }
 
 // the first `n` of them (n may be <= 0); zeros behind
@@ -104,8 +123,10 @@ __device__ __forceinline__ void adamw_element(const AdamwScalars& h,
 }
 
 // 28 bytes an fp32 element (22 a 16-bit one) and some 30 operations: bound
-// by memory.  All loads of a chunk are issued before the first is used.
-template <typename T>
+// by memory.  All loads of a chunk are issued before the first is used (the
+// barrier keeps the compiler from holding some back to save registers).
+// 2e8 bf16 weights: 803 us, 5.5 TB/s, where a copy of 4 GB reaches 4.75.
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(
     const AdamwTable tab, const AdamwScalars h, const float* norm) {
   constexpr int V = 16 / sizeof(T);
@@ -116,40 +137,47 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(
   float* m = (float*)tab.m[t] + at;
   float* v = (float*)tab.v[t] + at;
   const float coef = clip_coef(norm, h.max_norm);
-  float gf[NV][V], pf[NV][V], mf[NV][V], vf[NV][V], r;
+  float gf[V], pf[V], mf[V], vf[V], r;
   const int i0 = threadIdx.x * V;
-  if (left >= CHUNK) {
+  if (left == CHUNK) {
+    Raw<T, V> gr[NV], pr[NV];
+    Raw<float, V> mr[NV], vr[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int i = i0 + j * THREADS * V;
-      load_vec(g + i, gf[j]);
-      load_vec(p + i, pf[j]);
-      load_vec(m + i, mf[j]);
-      load_vec(v + i, vf[j]);
+      gr[j].template load<ONCE>(g + i);
+      pr[j].template load<ONCE>(p + i);
+      mr[j].template load<ONCE>(m + i);
+      vr[j].template load<ONCE>(v + i);
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int i = i0 + j * THREADS * V;
+      gr[j].floats(gf);
+      pr[j].floats(pf);
+      mr[j].floats(mf);
+      vr[j].floats(vf);
 #pragma unroll
       for (int k = 0; k < V; ++k)
-        adamw_element(h, coef, gf[j][k], pf[j][k], mf[j][k], vf[j][k], r);
-      store_vec(p + i, pf[j]);
-      store_vec(m + i, mf[j]);
-      store_vec(v + i, vf[j]);
+        adamw_element(h, coef, gf[k], pf[k], mf[k], vf[k], r);
+      store_vec<ONCE>(p + i, pf);
+      store_vec<ONCE>(m + i, mf);
+      store_vec<ONCE>(v + i, vf);
     }
   } else {
     for (int i = i0; i < left; i += THREADS * V) {
       const int n = left - i;
-      load_part(g + i, gf[0], n);
-      load_part(p + i, pf[0], n);
-      load_part(m + i, mf[0], n);
-      load_part(v + i, vf[0], n);
+      load_part(g + i, gf, n);
+      load_part(p + i, pf, n);
+      load_part(m + i, mf, n);
+      load_part(v + i, vf, n);
 #pragma unroll
       for (int k = 0; k < V; ++k)
-        adamw_element(h, coef, gf[0][k], pf[0][k], mf[0][k], vf[0][k], r);
-      store_part(p + i, pf[0], n);
-      store_part(m + i, mf[0], n);
-      store_part(v + i, vf[0], n);
+        adamw_element(h, coef, gf[k], pf[k], mf[k], vf[k], r);
+      store_part(p + i, pf, n);
+      store_part(m + i, mf, n);
+      store_part(v + i, vf, n);
     }
   }
 }
@@ -223,10 +251,14 @@ __device__ __forceinline__ uint2 pack_m(const float (&q)[8]) {
 }
 
 // bytes [0, n) of a code word, zeros behind
+typedef uint32_t word2 __attribute__((ext_vector_type(2), aligned(1)));
+template <bool ONCE>
 __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
   uint2 w = make_uint2(0, 0);
   if (n >= 8) {
-    __builtin_memcpy(&w, p, 8);
+    const word2 x = ONCE ? __builtin_nontemporal_load((const word2*)p)
+                         : *(const word2*)p;
+    w = make_uint2(x.x, x.y);
   } else {
     for (int k = 0; k < n; ++k) {
       const uint32_t b = p[k];
@@ -248,8 +280,12 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint2 w, int n) {
 
 // 16 lanes share a block of 256 elements: lane l holds elements l*8.. of
 // each half, so that a wave reads whole lines and the block's maximum needs
-// no shared memory (four DPP steps).
-template <typename T>
+// no shared memory (four DPP steps).  16 bytes an fp32 element (10 a 16-bit
+// one) against some 60 operations, which leaves the vector units little to
+// spare: with a correctly rounded root and quotient they were the limit (2e8
+// bf16 weights 430 us, with the hardware's 380, 5.3 TB/s).  Codes go through
+// the caches in any case: their next reader may find them there.
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(THREADS) void adamw8_kernel(
     const AdamwTable tab, const AdamwScalars h, const float* norm,
     uint32_t seed) {
@@ -260,26 +296,34 @@ __global__ __launch_bounds__(THREADS) void adamw8_kernel(
   uint8_t* v = (uint8_t*)tab.v[t] + at;
   const int b = threadIdx.x / 16, l = threadIdx.x % 16;
   float2* scale = (float2*)tab.s[t] + at / QBLOCK + b;
-  const bool full = left >= CHUNK;
+  const bool full = left == CHUNK;
   const float coef = clip_coef(norm, h.max_norm);
   const int i0 = b * QBLOCK + l * 8;
   const bool live = b * QBLOCK < left;  // the same for the 16 lanes
   float pf[2][8], gf[2][8], mf[2][8], rf[2][8];
   uint2 mc[2], vc[2];
   const float2 s = live ? *scale : make_float2(0.f, 0.f);
+  if (full) {
+    Raw<T, 8> gr[2], pr[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = i0 + j * 128;
-    if (full) {
-      load_vec(g + i, gf[j]);
-      load_vec(p + i, pf[j]);
-      mc[j] = load_codes(m + i, 8);
-      vc[j] = load_codes(v + i, 8);
-    } else {
+    for (int j = 0; j < 2; ++j) {
+      const int i = i0 + j * 128;
+      gr[j].template load<ONCE>(g + i);
+      pr[j].template load<ONCE>(p + i);
+      mc[j] = load_codes<false>(m + i, 8);
+      vc[j] = load_codes<false>(v + i, 8);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) gr[j].floats(gf[j]), pr[j].floats(pf[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = i0 + j * 128;
       load_part(g + i, gf[j], left - i);
       load_part(p + i, pf[j], left - i);
-      mc[j] = load_codes(m + i, left - i);
-      vc[j] = load_codes(v + i, left - i);
+      mc[j] = load_codes<false>(m + i, left - i);
+      vc[j] = load_codes<false>(v + i, left - i);
     }
   }
   uint32_t top_m = __float_as_uint(TINY), top_r = __float_as_uint(TINY);
@@ -317,7 +361,7 @@ __global__ __launch_bounds__(THREADS) void adamw8_kernel(
     }
     const uint2 mw = pack_m(mf[j]);
     if (full) {
-      store_vec(p + i, pf[j]);
+      store_vec<ONCE>(p + i, pf[j]);
       store_codes(m + i, mw, 8);
       store_codes(v + i, make_uint2(w[0], w[1]), 8);
     } else {
@@ -339,8 +383,8 @@ __global__ __launch_bounds__(THREADS) void adamw8_values_kernel(
     const int i = (j * THREADS + threadIdx.x) * 8;
     const int n = left - i;
     if (n <= 0) break;
-    const uint2 mc = load_codes((const uint8_t*)tab.m[t] + at + i, n);
-    const uint2 vc = load_codes((const uint8_t*)tab.v[t] + at + i, n);
+    const uint2 mc = load_codes<true>((const uint8_t*)tab.m[t] + at + i, n);
+    const uint2 vc = load_codes<true>((const uint8_t*)tab.v[t] + at + i, n);
     const float2 s = ((const float2*)tab.s[t])[(at + i) / QBLOCK];
     float m[8], v[8];
     decode8(mc, vc, m, v);
@@ -353,8 +397,8 @@ __global__ __launch_bounds__(THREADS) void adamw8_values_kernel(
     T* om = (T*)tab.p[t] + at + i;
     T* ov = (T*)const_cast<void*>(tab.g[t]) + at + i;
     if (n >= 8) {
-      store_vec(om, m);
-      store_vec(ov, v);
+      store_vec<true>(om, m);
+      store_vec<true>(ov, v);
     } else {
       store_part(om, m, n);
       store_part(ov, v, n);
@@ -366,26 +410,34 @@ __global__ __launch_bounds__(THREADS) void adamw8_values_kernel(
 // Squares and sums in 64 bits: a square of a 32-bit value is exact there,
 // and the order of the sum does not reach the 32-bit result.  Read-bound:
 // 4 (2) bytes an element.
-template <typename T>
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(THREADS) void sumsq_kernel(
     const GradTable tab, double* __restrict__ partial) {
   constexpr int V = 16 / sizeof(T);
   constexpr int NV = CHUNK / (THREADS * V);
   double acc = 0.0;
+  float gf[V];
   for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
     const auto [t, at, left] = find_chunk(tab, c);
     const T* g = (const T*)tab.g[t] + at + threadIdx.x * V;
-    const int n = left - threadIdx.x * V;
-    float gf[NV][V];
+    if (left == CHUNK) {
+      Raw<T, V> r[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (left == CHUNK) load_vec(g + j * THREADS * V, gf[j]);
-      else load_part(g + j * THREADS * V, gf[j], n - j * THREADS * V);
+      for (int j = 0; j < NV; ++j) r[j].template load<ONCE>(g + j * THREADS * V);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        r[j].floats(gf);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc += (double)gf[k] * (double)gf[k];
+      }
+    } else {
+      for (int i = threadIdx.x * V; i < left; i += THREADS * V) {
+        load_part((const T*)tab.g[t] + at + i, gf, left - i);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc += (double)gf[k] * (double)gf[k];
+      }
     }
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int k = 0; k < V; ++k) acc += (double)gf[j][k] * (double)gf[j][k];
   }
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, WAVE);
   __shared__ double part[THREADS / WAVE];
@@ -410,14 +462,22 @@ __global__ __launch_bounds__(THREADS) void norm_final_kernel(
 
 template <typename T>
 void go_adamw(hipStream_t s, const AdamwTable& tab, const AdamwScalars& h,
-              const float* norm) {
-  adamw_kernel<T><<<dim3(tab.chunks), THREADS, 0, s>>>(tab, h, norm);
+              const float* norm, bool once) {
+  if (once)
+    adamw_kernel<T, true><<<dim3(tab.chunks), THREADS, 0, s>>>(tab, h, norm);
+  else
+    adamw_kernel<T, false><<<dim3(tab.chunks), THREADS, 0, s>>>(tab, h, norm);
 }
 
 template <typename T>
 void go_adamw8(hipStream_t s, const AdamwTable& tab, const AdamwScalars& h,
-               const float* norm, uint32_t seed) {
-  adamw8_kernel<T><<<dim3(tab.chunks), THREADS, 0, s>>>(tab, h, norm, seed);
+               const float* norm, bool once, uint32_t seed) {
+  if (once)
+    adamw8_kernel<T, true>
+        <<<dim3(tab.chunks), THREADS, 0, s>>>(tab, h, norm, seed);
+  else
+    adamw8_kernel<T, false>
+        <<<dim3(tab.chunks), THREADS, 0, s>>>(tab, h, norm, seed);
 }
 
 template <typename T>
@@ -427,8 +487,11 @@ void go_values(hipStream_t s, const AdamwTable& tab) {
 
 template <typename T>
 void go_sumsq(hipStream_t s, const GradTable& tab, double* partial,
-              int blocks) {
-  sumsq_kernel<T><<<dim3(blocks), THREADS, 0, s>>>(tab, partial);
+              int blocks, bool once) {
+  if (once)
+    sumsq_kernel<T, true><<<dim3(blocks), THREADS, 0, s>>>(tab, partial);
+  else
+    sumsq_kernel<T, false><<<dim3(blocks), THREADS, 0, s>>>(tab, partial);
 }
 
 #define BY_DTYPE(dtype, fn, ...)                        \
@@ -443,18 +506,19 @@ void go_sumsq(hipStream_t s, const GradTable& tab, double* partial,
 
 extern "C" int launch_adamw(void* stream, const AdamwTable* tab,
                             const AdamwScalars* h, const float* norm,
-                            int dtype) {
+                            int dtype, bool once) {
   if (tab->chunks == 0) return 0;
-  BY_DTYPE(dtype, go_adamw, (hipStream_t)stream, *tab, *h, norm)
+  BY_DTYPE(dtype, go_adamw, (hipStream_t)stream, *tab, *h, norm, once)
   HIP_CHECK_LAST();
   return 0;
 }
 
 extern "C" int launch_adamw8(void* stream, const AdamwTable* tab,
                              const AdamwScalars* h, const float* norm,
-                             int dtype, uint32_t seed) {
+                             int dtype, bool once, uint32_t seed) {
   if (tab->chunks == 0) return 0;
-  BY_DTYPE(dtype, go_adamw8, (hipStream_t)stream, *tab, *h, norm, seed)
+  BY_DTYPE(dtype, go_adamw8, (hipStream_t)stream, *tab, *h, norm, once,
+           seed)
   HIP_CHECK_LAST();
   return 0;
 }
@@ -468,9 +532,9 @@ extern "C" int launch_adamw8_values(void* stream, const AdamwTable* tab,
 }
 
 extern "C" int launch_sumsq(void* stream, const GradTable* tab, int dtype,
-                            double* partial, int blocks) {
+                            double* partial, int blocks, bool once) {
   if (tab->chunks == 0 || blocks == 0) return 0;
-  BY_DTYPE(dtype, go_sumsq, (hipStream_t)stream, *tab, partial, blocks)
+  BY_DTYPE(dtype, go_sumsq, (hipStream_t)stream, *tab, partial, blocks, once)
   HIP_CHECK_LAST();
   return 0;
 }

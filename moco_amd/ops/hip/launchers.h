@@ -91,16 +91,17 @@ struct AdamwScalars {
   float beta1, one_minus_beta1, beta2, one_minus_beta2;
   float inv_root_bc2, eps, decay, step_size, max_norm;
 };
-// norm: device fp32 scalar for the clip, or null for none
+// norm: device fp32 scalar for the clip, or null for none; once: the data go
+// past the caches
 int launch_adamw(void* stream, const AdamwTable* tab, const AdamwScalars* h,
-                 const float* norm, int dtype);
+                 const float* norm, int dtype, bool once);
 int launch_adamw8(void* stream, const AdamwTable* tab, const AdamwScalars* h,
-                  const float* norm, int dtype, uint32_t seed);
+                  const float* norm, int dtype, bool once, uint32_t seed);
 // decoded moments of the codes m, v, s into p (m) and g (v), of type dtype
 int launch_adamw8_values(void* stream, const AdamwTable* tab, int dtype);
 // partial[blocks]: sums of squares of the table's g
 int launch_sumsq(void* stream, const GradTable* tab, int dtype,
-                 double* partial, int blocks);
+                 double* partial, int blocks, bool once);
 // out = sqrt(sum of partial[0..n))
 int launch_norm_final(void* stream, const double* partial, int n, float* out);
 
