@@ -50,8 +50,10 @@ def force_fallback() -> bool:
 
 def use_hip(*tensors) -> bool:
     """True when these tensors should run on the HIP kernels."""
-    on_gpu = any(t.is_cuda for t in tensors if isinstance(t, torch.Tensor))
-    if not on_gpu:
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.is_cuda:
+            break
+    else:
         return False
     if force_fallback():
         return False

@@ -796,30 +796,31 @@ std::vector<torch::Tensor> norm_residual_bwd(
     o.d_gate = out[2].data_ptr();
   }
   const OptTensor* vec[5] = {&w1, &b1, &w2, &b2, &scale};
-  const int blocks = norm_bwd_blocks(&c.a);
-  const int64_t slab = (int64_t)blocks * c.a.width;
-  int vecs = 0;
-  for (int j = 0; j < 5; ++j)
-    vecs += ((want >> (3 + j)) & 1) && vec[j]->has_value();
-  auto partial = new_tensor({vecs * slab}, torch::kFloat32, x.device());
-  NormColumns cols{};
-  int used = 0;
+  void** d_vec[5] = {&o.d_w1, &o.d_b1, &o.d_w2, &o.d_b2, &o.d_scale};
   for (int j = 0; j < 5; ++j) {
     if (!((want >> (3 + j)) & 1) || !vec[j]->has_value()) continue;
     auto& d = out[3 + j];
-    // no rows: nothing is launched, and the sums are zero
     d = new_tensor({c.a.width}, (*vec[j])->scalar_type(), x.device());
+    *d_vec[j] = d.data_ptr();
+    // no rows: nothing is launched, and the sums are zero
     if (!c.a.rows) d.zero_();
-    o.partial[j] = partial.data_ptr<float>() + used * slab;
-    cols.partial[used] = o.partial[j];
-    cols.out[used] = d.data_ptr();
-    cols.dtype[used++] = adamw_dtype(d, "weights, biases and scale");
   }
-  if (c.a.rows) {
-    CHECK_LAUNCH(launch_norm_bwd(cur_stream(), &c.a, &o, blocks));
-    CHECK_LAUNCH(launch_norm_columns(cur_stream(), &cols, vecs, blocks,
-                                     c.a.width));
+  if (!c.a.rows) return out;
+  const bool sums[4] = {o.d_w1 || o.d_scale,
+                        o.d_b1 || (o.d_scale && c.a.b1), o.d_w2 != nullptr,
+                        o.d_b2 != nullptr};
+  const int n = sums[0] + sums[1] + sums[2] + sums[3];
+  const int blocks = norm_bwd_blocks(&c.a);
+  const int64_t slab = (int64_t)blocks * c.a.width;
+  torch::Tensor partial;
+  if (n) {
+    partial = new_tensor({n * slab}, torch::kFloat32, x.device());
+    float* at = partial.data_ptr<float>();
+    for (int j = 0; j < 4; ++j)
+      if (sums[j]) o.partial[j] = at, at += slab;
   }
+  CHECK_LAUNCH(launch_norm_bwd(cur_stream(), &c.a, &o, blocks));
+  if (n) CHECK_LAUNCH(launch_norm_columns(cur_stream(), &c.a, &o, blocks));
   return out;
 }
 

@@ -125,24 +125,20 @@ struct NormArgs {
   float scale_value, post_eps, pre_eps;
 };
 // d_r, d_y: contiguous, null where an output has no gradient; d_x, d_h,
-// d_gate: null where none is wanted; partial[j]: fp32 [blocks, width] for
-// the column sums of dw1, db1, dw2, db2, dscale, null where none is wanted
+// d_gate and the vectors' (of their vector's type): null where none is
+// wanted; partial[j]: fp32 [blocks, width] for column sum j (0 and 1 for d_w1,
+// d_b1, d_scale; 2 for d_w2; 3 for d_b2), null where it is not needed
 struct NormGrads {
   const void *d_r, *d_y;
-  void *d_x, *d_h, *d_gate;
-  float* partial[5];
-};
-struct NormColumns {
-  const float* partial[5];
-  void* out[5];
-  int dtype[5];
+  void *d_x, *d_h, *d_gate, *d_w1, *d_b1, *d_w2, *d_b2, *d_scale;
+  float* partial[4];
 };
 int launch_norm_fwd(void* stream, const NormArgs* a);
 int norm_bwd_blocks(const NormArgs* a);
 int launch_norm_bwd(void* stream, const NormArgs* a, const NormGrads* o,
                     int blocks);
-int launch_norm_columns(void* stream, const NormColumns* v, int vecs,
-                        int blocks, int64_t width);
+int launch_norm_columns(void* stream, const NormArgs* a, const NormGrads* o,
+                        int blocks);
 
 // ---- bn.hip ---------------------------------------------------------------
 // x/y/g/res: [R, C] bf16 (NHWC flattened); stats fp32; C in {64..256 dividing

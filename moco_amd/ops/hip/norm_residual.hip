@@ -15,8 +15,9 @@
 //   t  = d_y w2;   d = d_r + rstd_r (t - [mean t] - rhat mean(t rhat));  dx = d
 //   dn = d scale a;   dgate = act'(gate) d scale n (summed over a row's gate)
 //   t1 = dn w1;    dh = rstd_h (t1 - [mean t1] - hhat mean(t1 hhat))
-//   dw2 = sum d_y rhat, db2 = sum d_y, dw1 = sum dn hhat, db1 = sum dn,
-//   dscale = sum d a n      over rows; [..] only in a LayerNorm.
+//   over rows: S0 = sum d a hhat, S1 = sum d a, S2 = sum d_y rhat, S3 = sum d_y
+//   dw1 = scale S0, db1 = scale S1, dscale = w1 S0 + b1 S1, dw2 = S2, db2 = S3
+//   ([..], S1 and S3 only with a LayerNorm)
 //
 // Both directions are bound by memory: each input is read and each output
 // written once.  NT threads share a row, 8 neighbouring elements a thread
@@ -378,9 +379,8 @@ __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_fwd_kernel(
   }
 }
 
-// Column sums of a workgroup, in the order of NormGrads::partial: dw1, db1,
-// dw2, db2, dscale.
-constexpr int VECS = 5;
+// Column sums of a workgroup, S0 to S3
+constexpr int SUMS = 4;
 
 // LAYER: whether one norm is a LayerNorm (or has a bias).  What bounds this
 // pass after memory is the number of vector instructions, some 50 an element,
@@ -440,9 +440,9 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
       fetch(which, k, v);
     }
   };
-  float acc[VECS][K][V];
+  float acc[SUMS][K][V];
 #pragma unroll
-  for (int j = 0; j < VECS; ++j)
+  for (int j = 0; j < SUMS; ++j)
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -571,13 +571,11 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
       vec(1, k, s);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float dsn = d[k][i] * nf[i];
-        acc[4][k][i] += dsn * act[i];
-        slope[i] *= dsn * s[i];
-        const float dn = d[k][i] * (s[i] * act[i]);
-        acc[0][k][i] += dn * hat_h(k, i);
-        if (LAYER) acc[1][k][i] += dn;
-        d[k][i] = dn * w[i];  // t1 from here on
+        const float da = d[k][i] * act[i];
+        slope[i] *= d[k][i] * s[i] * nf[i];
+        acc[0][k][i] += da * hat_h(k, i);
+        if (LAYER) acc[1][k][i] += da;
+        d[k][i] = da * s[i] * w[i];  // t1 from here on
         const float t1 = i >= c[k].skip ? d[k][i] : 0.f;
         q[0] += t1 * hat_h(k, i);
         if (LAYER) q[1] += t1;
@@ -608,7 +606,7 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
   }
   // the workgroup's column sums: its groups' are added in LDS first
 #pragma unroll
-  for (int j = 0; j < VECS; ++j) {
+  for (int j = 0; j < SUMS; ++j) {
     if (o.partial[j] == nullptr) continue;
     float* out = o.partial[j] + (int64_t)blockIdx.x * a.width;
     if constexpr (GROUPS > 1) {
@@ -630,38 +628,75 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
   }
 }
 
-// out[c] = sum over blocks of partial[b][c], for up to VECS vectors; one
-// workgroup adds 32 columns (a line of memory), 32 parts of the blocks side
-// by side with 8 loads each on their way (16 parts and one load at a time
-// took 10 us for 512 blocks of any width)
+__device__ __forceinline__ void store_any(void* p, int type, int c, float f) {
+  switch (type) {
+    case 0: ((float*)p)[c] = f; break;
+    case 1: ((__bf16*)p)[c] = (__bf16)f; break;
+    default: ((_Float16*)p)[c] = (_Float16)f; break;
+  }
+}
+
+// a vector of fp32 or the block's type, or a constant
+__device__ __forceinline__ float load_any(const void* p, int type, int c,
+                                          float none) {
+  if (p == nullptr) return none;
+  return type == 0   ? ((const float*)p)[c]
+         : type == 1 ? (float)((const __bf16*)p)[c]
+                     : (float)((const _Float16*)p)[c];
+}
+
+// The workgroups' column sums added, and the vectors' gradients of them.  A
+// workgroup has 32 columns (a line of memory) and adds S0 and S1, or S2 and
+// S3; 32 parts of the rows of partial sums side by side with 8 loads each on
+// their way (16 parts and one load at a time took 10 us for 512 rows of any
+// width).
 __global__ __launch_bounds__(1024) void norm_columns_kernel(
-    const NormColumns v, int blocks, int width) {
+    const NormArgs a, const NormGrads o, int blocks) {
   const int lane = threadIdx.x % 32, part = threadIdx.x / 32;
-  const int c = min((int)blockIdx.x * 32 + lane, width - 1);
-  const float* p = v.partial[blockIdx.y] + c;
-  float s = 0.f;
-  int b = part;
-  for (; b + 7 * 32 < blocks; b += 8 * 32) {
-    float f[8];
+  const bool in = (int)blockIdx.x * 32 + lane < a.width;
+  const int c = in ? blockIdx.x * 32 + lane : a.width - 1;
+  const int first = 2 * blockIdx.y;
+  __shared__ float lds[2][32][33];
+  for (int j = 0; j < 2; ++j) {
+    const float* p = o.partial[first + j];
+    float s = 0.f;
+    if (p != nullptr) {
+      p += c;
+      int b = part;
+      for (; b + 7 * 32 < blocks; b += 8 * 32) {
+        float f[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = p[(int64_t)(b + j * 32) * width];
+        for (int i = 0; i < 8; ++i) f[i] = p[(int64_t)(b + i * 32) * a.width];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += f[j];
+        for (int i = 0; i < 8; ++i) s += f[i];
+      }
+      for (; b < blocks; b += 32) s += p[(int64_t)b * a.width];
+    }
+    lds[j][part][lane] = s;
   }
-  for (; b < blocks; b += 32) s += p[(int64_t)b * width];
-  __shared__ float lds[32][33];
-  lds[part][lane] = s;
   __syncthreads();
-  if (part != 0 || (int)blockIdx.x * 32 + lane >= width) return;
-  s = 0.f;
+  if (part != 0 || !in) return;
+  float s[2] = {0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < 32; ++j) s += lds[j][lane];
-  void* out = v.out[blockIdx.y];
-  switch (v.dtype[blockIdx.y]) {
-    case 0: ((float*)out)[c] = s; break;
-    case 1: ((__bf16*)out)[c] = (__bf16)s; break;
-    default: ((_Float16*)out)[c] = (_Float16)s; break;
+  for (int j = 0; j < 32; ++j) {
+    s[0] += lds[0][j][lane];
+    s[1] += lds[1][j][lane];
   }
+  const int t = a.type_h;
+  auto type = [&](int bit) { return a.f32 >> bit & 1 ? 0 : t; };
+  if (first) {
+    if (o.d_w2 != nullptr) store_any(o.d_w2, type(2), c, s[0]);
+    if (o.d_b2 != nullptr) store_any(o.d_b2, type(3), c, s[1]);
+    return;
+  }
+  const float w = load_any(a.w1, type(0), c, 1.f);
+  const float b = load_any(a.b1, type(1), c, 0.f);
+  const float scale = load_any(a.scale, type(4), c, a.scale_value);
+  if (o.d_w1 != nullptr) store_any(o.d_w1, type(0), c, scale * s[0]);
+  if (o.d_b1 != nullptr) store_any(o.d_b1, type(1), c, scale * s[1]);
+  if (o.d_scale != nullptr)
+    store_any(o.d_scale, type(4), c,
+              a.b1 != nullptr ? w * s[0] + b * s[1] : w * s[0]);
 }
 
 template <typename TX, typename TH, int NT, int K, int V>
@@ -751,11 +786,10 @@ extern "C" int launch_norm_bwd(void* stream, const NormArgs* a,
   return go_types((hipStream_t)stream, *a, o, blocks);
 }
 
-extern "C" int launch_norm_columns(void* stream, const NormColumns* v,
-                                   int vecs, int blocks, int64_t width) {
-  if (vecs == 0 || width == 0) return 0;
-  norm_columns_kernel<<<dim3((unsigned)((width + 31) / 32), vecs), 1024, 0,
-                        (hipStream_t)stream>>>(*v, blocks, (int)width);
+extern "C" int launch_norm_columns(void* stream, const NormArgs* a,
+                                   const NormGrads* o, int blocks) {
+  norm_columns_kernel<<<dim3((unsigned)((a->width + 31) / 32), 2), 1024, 0,
+                        (hipStream_t)stream>>>(*a, *o, blocks);
   HIP_CHECK_LAST();
   return 0;
 }
