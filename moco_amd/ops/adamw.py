@@ -223,8 +223,8 @@ def _adamw(params, grads, ms, vs, scales, step, lr, betas, eps, weight_decay,
     params, grads = list(params), list(grads)
     if use_hip(*params[:1]):
         return ext().adamw_step(
-            params, grads, ms, vs, scales, int(step), lr, betas[0], betas[1], eps,
-            weight_decay, max_norm, total_norm, seed & 0xFFFFFFFF)
+            params, grads, ms, vs, scales, int(step), lr, betas[0], betas[1],
+            eps, weight_decay, max_norm, total_norm, seed & 0xFFFFFFFF)
     _check_lists(params, grads, ms, vs, scales)
     if not params:
         return total_norm

@@ -5,7 +5,8 @@
 //
 //   g  = coef * grad              coef = min(1, max_norm / (norm + 1e-6))
 //   m' = b1 m + (1 - b1) g        v' = b2 v + (1 - b2) g^2
-//   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//   p' = p (1 - lr wd)
+//        - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
 // Each operation is rounded by itself (no contraction into fma), as a plain
 // elementwise program in 32 bits does, so that what is rounded to 8 bits
@@ -423,7 +424,8 @@ __global__ __launch_bounds__(THREADS) void sumsq_kernel(
     if (left == CHUNK) {
       Raw<T, V> r[NV];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) r[j].template load<ONCE>(g + j * THREADS * V);
+      for (int j = 0; j < NV; ++j)
+        r[j].template load<ONCE>(g + j * THREADS * V);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {

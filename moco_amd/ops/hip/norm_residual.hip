@@ -34,9 +34,9 @@
 namespace {
 
 constexpr int BLOCK = 256;  // threads of a workgroup, at least
-#ifndef NORM_FWD_THREADS
-#define NORM_FWD_THREADS (256 * 1024)
-#endif
+// threads of a forward grid at most: 1024 on each of 256 CUs, which is what
+// their registers let be there at once; beyond that workgroups take more rows
+constexpr int FWD_THREADS = 256 * 1024;
 
 // V elements as they lie in memory: registers hold whole words until an
 // element is used, so that several loads are on their way at once
@@ -274,9 +274,11 @@ struct FwdRow {
   }
 };
 
-// LAYER: whether one norm is a LayerNorm.  A workgroup keeps its columns' weights in
-// registers (K = 1) over its rows, and the next row's inputs are on their way
-// while this one's sums are taken.
+// LAYER: whether one norm is a LayerNorm.  A workgroup keeps its columns'
+// weights in registers (K = 1) over its rows, and the next row's inputs are on
+// their way while this one's sums are taken.  16384 x 4096 bf16, gated: 125
+// us, 5.4 TB/s, where a copy of 4 GB reaches 4.75 (one row a workgroup, its
+// weights read each time: 170 us).
 template <typename TX, typename TH, int NT, int K, int V, bool LAYER>
 __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_fwd_kernel(
     const NormArgs a) {
@@ -330,8 +332,8 @@ __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_fwd_kernel(
         for (int i = 0; i < V; ++i) f[k][i] = cur.h[k][i];
       float mean = 0.f, rstd = 1.f;
       if (a.post != NORM_NONE) {
-        row_stats<NT, K, V, LAYER>(f, c, a.post, inv_c, a.post_eps, sum, turn, mean,
-                            rstd);
+        row_stats<NT, K, V, LAYER>(f, c, a.post, inv_c, a.post_eps, sum, turn,
+                                   mean, rstd);
         if (t == 0 && in && a.stats != nullptr) {
           a.stats[row] = mean;
           a.stats[a.rows + row] = rstd;
@@ -361,7 +363,8 @@ __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_fwd_kernel(
     }
     if (a.pre == NORM_NONE) continue;
     float mean, rstd;
-    row_stats<NT, K, V, LAYER>(f, c, a.pre, inv_c, a.pre_eps, sum, turn, mean, rstd);
+    row_stats<NT, K, V, LAYER>(f, c, a.pre, inv_c, a.pre_eps, sum, turn, mean,
+                               rstd);
     if (t == 0 && in && a.stats != nullptr) {
       a.stats[2 * a.rows + row] = mean;
       a.stats[3 * a.rows + row] = rstd;
@@ -386,7 +389,11 @@ constexpr int SUMS = 4;
 // pass after memory is the number of vector instructions, some 50 an element,
 // and registers, which bound how many rows are on their way per CU.  So hats
 // and weighted values are made again rather than kept, and the weights are
-// read from LDS (K = 1), where a workgroup puts them once.
+// read from LDS (K = 1), where a workgroup puts them once.  16384 x 4096
+// bf16, gated: 220 us, 4.9 TB/s (321 us with twice the instructions and the
+// weights from L2).  Above 8192 columns (K = 2) the registers do not suffice
+// for two vectors a thread, and some are spilled: 2048 x 16384 283 us, 1.9
+// TB/s.
 template <typename TX, typename TH, int NT, int K, int V, bool LAYER>
 __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT,
                              NT < WAVE || (LAYER && NT < 1024) ? 3 : 4) void
@@ -394,8 +401,9 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
   constexpr int GROUPS = NT < BLOCK ? BLOCK / NT : 1;
   constexpr bool KEEP = K == 1;
   constexpr int KEPT = LAYER ? 4 : 3;  // w1, scale, w2, b1
-  __shared__ RowSum<NT, 2> sums2[GROUPS];
-  __shared__ RowSum<NT, 3> sums3[GROUPS];
+  constexpr int P = LAYER ? 2 : 1, Q3 = LAYER ? 3 : 2;  // row sums of a step
+  __shared__ RowSum<NT, P> pre_sums[GROUPS];
+  __shared__ RowSum<NT, Q3> post_sums[GROUPS];
   // [vector][four elements][thread]: neighbouring threads' reads of 16 bytes
   // lie side by side
   constexpr int Q = V >= 4 ? V / 4 : 1, W = V / Q;
@@ -404,8 +412,8 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
                          [GROUPS > 1 ? NT * K * V : 1];
   const int group = group_of<NT>();
   const int t = threadIdx.x % NT;
-  RowSum<NT, 2>& sum2 = sums2[group];
-  RowSum<NT, 3>& sum3 = sums3[group];
+  RowSum<NT, P>& pre_sum = pre_sums[group];
+  RowSum<NT, Q3>& post_sum = post_sums[group];
   const float inv_c = 1.f / (float)a.width;
   const bool full = a.gate_kind == NORM_GATE_FULL;
   const bool per_row = a.gate_kind == NORM_GATE_ROW;
@@ -494,7 +502,7 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
       return (LAYER ? h[k][i] - mean_h : h[k][i]) * rstd_h;
     };
     // the norm before the next block: its row sums need r
-    float p[2] = {0.f, 0.f};
+    float p[P] = {};
     if (o.d_y != nullptr) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -525,12 +533,12 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
           acc[2][k][i] += dy[k][i] * d[k][i];
           if (LAYER) acc[3][k][i] += dy[k][i];
           p[0] += tt * d[k][i];
-          if (LAYER) p[1] += tt;
+          if constexpr (LAYER) p[1] += tt;
         }
       }
-      sum2(p, turn);
+      pre_sum(p, turn);
       p[0] *= inv_c;
-      p[1] = LAYER && a.pre == NORM_LAYER ? p[1] * inv_c : 0.f;
+      if constexpr (LAYER) p[1] = a.pre == NORM_LAYER ? p[1] * inv_c : 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float v[V];
@@ -538,7 +546,7 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float back = dy[k][i] * v[i] - d[k][i] * p[0];
-          d[k][i] = dr[k][i] + rstd_r * (LAYER ? back - p[1] : back);
+          d[k][i] = dr[k][i] + rstd_r * (LAYER ? back - p[P - 1] : back);
         }
       }
     } else {
@@ -554,7 +562,7 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
     }
     if (a.h == nullptr) continue;
     // the gate, the scale and the norm after the block
-    float q[3] = {0.f, 0.f, 0.f};
+    float q[Q3] = {};  // of t1 hhat, of the gate, of t1
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float w[V], s[V], nf[V];
@@ -578,22 +586,23 @@ norm_bwd_kernel(const NormArgs a, const NormGrads o) {
         d[k][i] = da * s[i] * w[i];  // t1 from here on
         const float t1 = i >= c[k].skip ? d[k][i] : 0.f;
         q[0] += t1 * hat_h(k, i);
-        if (LAYER) q[1] += t1;
+        if constexpr (LAYER) q[2] += t1;
       }
       if (full && o.d_gate != nullptr && in)
         store_f<TH>(o.d_gate, row * a.width, c[k], slope);
       if (per_row) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          q[2] += i >= c[k].skip ? slope[i] : 0.f;
+          q[1] += i >= c[k].skip ? slope[i] : 0.f;
       }
     }
-    if (a.post != NORM_NONE || per_row) sum3(q, turn);
+    if (a.post != NORM_NONE || per_row) post_sum(q, turn);
     if (per_row && o.d_gate != nullptr && t == 0 && in)
-      ((TH*)o.d_gate)[row] = (TH)(q[2] * row_slope[0]);
+      ((TH*)o.d_gate)[row] = (TH)(q[1] * row_slope[0]);
     if (o.d_h == nullptr || !in) continue;
     const float m1 = a.post != NORM_NONE ? q[0] * inv_c : 0.f;
-    const float m0 = LAYER && a.post == NORM_LAYER ? q[1] * inv_c : 0.f;
+    const float m0 =
+        LAYER && a.post == NORM_LAYER ? q[Q3 - 1] * inv_c : 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -706,7 +715,7 @@ void go(hipStream_t s, const NormArgs& a, const NormGrads* o, int blocks) {
   const bool layer = a.post == NORM_LAYER || a.pre == NORM_LAYER;
   if (o == nullptr) {
     const int64_t grid = std::min<int64_t>((a.rows + GROUPS - 1) / GROUPS,
-                                           NORM_FWD_THREADS / THREADS);
+                                           FWD_THREADS / THREADS);
     if (layer)
       norm_fwd_kernel<TX, TH, NT, K, V, true>
           <<<dim3((unsigned)grid), THREADS, 0, s>>>(a);
@@ -722,6 +731,10 @@ void go(hipStream_t s, const NormArgs& a, const NormGrads* o, int blocks) {
   }
 }
 
+// 8 elements a thread, and the fewest threads a row that hold it: narrow rows
+// share waves (65536 x 64: 18 us backward, a wave a row 76), wide ones spread
+// over up to 16 (4096 columns over 512 threads: 2 rows on their way per CU
+// where 256 threads with twice the registers had 1).
 template <typename TX, typename TH>
 int go_width(hipStream_t s, const NormArgs& a, const NormGrads* o,
              int blocks) {

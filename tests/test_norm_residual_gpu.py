@@ -181,7 +181,9 @@ def test_one_module_for_both_norms_and_one_element_scale():
 def run_graph(x, h, post, pre, leaves, d):
     from moco_amd.ops import norm_residual
     r, y = norm_residual(x, h, post=post, pre=pre, scale=0.5)
-    return (r, y, *torch.autograd.grad((r, y), leaves, d))
+    grads = torch.autograd.grad((r, y), leaves, d)
+    # without their graph, whose nodes would stay on this call's stream
+    return (r.detach(), y.detach(), *grads)
 
 
 def test_streams_graphs_and_repeatability():
