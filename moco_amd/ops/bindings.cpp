@@ -552,7 +552,8 @@ c10::optional<torch::Tensor> adamw_step(
   }
   // autograd's count of writes: a graph that saved a weight notices
   for (const Refs* list : {&params, &ms, &vs, &scales})
-    for (const auto* t : list->t) t->unsafeGetTensorImpl()->bump_version();
+    for (const auto* t : list->t)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return total_norm;
 }
 

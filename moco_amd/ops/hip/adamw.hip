@@ -9,9 +9,10 @@
 //        - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
 // Each operation is rounded by itself (no contraction into fma), as a plain
-// elementwise program in 32 bits does, so that what is rounded to 8 bits
-// afterwards falls on the same codes.  Root and reciprocal are the
-// hardware's, each off by an ulp at most.
+// elementwise program in 32 bits does, and the root is rounded correctly, so
+// that what is rounded to 8 bits afterwards falls on the same codes (a root
+// that is off by an ulp moves one code in 2e5, and with it later steps).  The
+// reciprocal, which reaches the weights alone, is the hardware's: an ulp.
 #include "common.h"
 #include "launchers.h"
 
@@ -118,7 +119,7 @@ __device__ __forceinline__ void adamw_element(const AdamwScalars& h,
   g = g * coef;
   m = m * h.beta1 + g * h.one_minus_beta1;
   v = v * h.beta2 + (g * g) * h.one_minus_beta2;
-  r = __builtin_amdgcn_sqrtf(v);
+  r = sqrtf(v);
   const float q = m * __builtin_amdgcn_rcpf(r * h.inv_root_bc2 + h.eps);
   p = p * h.decay - q * h.step_size;
 }
