@@ -5,8 +5,8 @@ import numpy as np
 import pytest
 import torch
 
-from adamw_oracle import (HALF, LEAST, check_codes, decode, mem, root_value,
-                          step64)
+from adamw_oracle import (HALF, LEAST, check_codes, decode, dither, mem,
+                          root_value, step64)
 
 pytestmark = pytest.mark.gpu
 
@@ -173,6 +173,41 @@ def test_rounding_to_e4m3_matches_torch():
     sm = st[3][0][:, 0].repeat_interleave(256).cpu()
     want = (g * sm.reciprocal()).clamp(-448, 448).to(torch.float8_e4m3fn)
     assert torch.equal(st[1][0].cpu().float(), want.float())
+
+
+def test_codes_are_those_of_32_bit_arithmetic():
+    """Bit for bit over three steps: numpy's float32 operations are each
+    rounded correctly, and so are the kernel's up to the codes (the quotient
+    after them is not, and is not looked at)."""
+    from moco_amd.ops import adamw8bit_
+    f = np.float32
+    n, b1, b2 = 100_003, 0.9, 0.999
+    rows = -(-n // 256)
+    st = make([(n,)], torch.float32, True)
+    m, r = np.zeros(rows * 256, f), np.zeros(rows * 256, f)
+    for step in range(1, 4):
+        gs = grads_for(st[0], step)
+        adamw8bit_(st[0], gs, *st[1:], step=step, seed=4, lr=1e-3,
+                   betas=(b1, b2))
+        g = np.zeros(rows * 256, f)
+        g[:n] = gs[0].cpu().numpy()
+        m = m * f(b1) + g * f(1 - b1)
+        r = np.sqrt((r * r) * f(b2) + (g * g) * f(1 - b2))
+        m, r = m.reshape(-1, 256), r.reshape(-1, 256)
+        sm = np.maximum(abs(m).max(1, keepdims=True), f(1e-30)) * f(1 / 448)
+        sr = np.maximum(r.max(1, keepdims=True), f(1e-30)) * f(1 / 1.9375)
+        assert np.array_equal(st[3][0].cpu().numpy(), np.hstack([sm, sr]))
+        mc = torch.from_numpy(np.clip(m * (f(1) / sm), f(-448), f(448))).to(
+            torch.float8_e4m3fn)
+        bits = (r * (f(1) / sr) * f(2.0 ** -112)).view(np.int32)
+        up = (dither(rows * 256, 0, step, 4) * 2 ** 19).astype(np.int32)
+        rc = np.minimum((bits + up.reshape(-1, 256)) >> 19, 255)
+        rc = np.where(r > 0, np.maximum(rc, 1), 0)
+        assert torch.equal(st[1][0].cpu().float(), mc.float().view(-1)[:n])
+        assert np.array_equal(st[2][0].cpu().numpy(), rc.reshape(-1)[:n])
+        m = (mc.float().numpy() * sm).reshape(-1)
+        r = ((rc.astype(np.int32) << 19).view(f) * f(2.0 ** 112)
+             * sr).reshape(-1)
 
 
 @pytest.mark.parametrize("dtype", list(HALF))
