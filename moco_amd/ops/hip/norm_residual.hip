@@ -76,15 +76,19 @@ struct Cols {
 };
 
 // off (to the row) is the same for a wave: it stays in scalar registers, and
-// one 32-bit offset serves all arrays of a type
+// one 32-bit offset serves all arrays of a type.  The empty asm keeps the
+// offset's widening to 64 bits beside the access, where it is part of the
+// instruction; moved out of the row loop it costs two registers an array (141
+// instead of 126 in the backward pass, a workgroup a CU less).
 template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> load_raw(const void* base, int64_t off,
                                               const Cols<V>& c,
                                               bool wanted = true) {
   Raw<T, V> r;
   if (wanted) {
-    const char* p = (const char*)base + off * (int64_t)sizeof(T) +
-                    c.col * (uint32_t)sizeof(T);
+    uint32_t at = c.col * (uint32_t)sizeof(T);
+    asm volatile("" : "+v"(at));
+    const char* p = (const char*)base + off * (int64_t)sizeof(T) + at;
     if constexpr (V * sizeof(T) < 4) {
       uint16_t u;
       __builtin_memcpy(&u, p, 2);
@@ -107,8 +111,9 @@ __device__ __forceinline__ void store_f(void* base, int64_t off,
   char* p = (char*)base + off * (int64_t)sizeof(T);
 #pragma unroll
   for (int i = 0; i < V; ++i) r[i] = (T)f[i];  // to nearest even
-  if (c.live())
-    __builtin_memcpy(p + c.col * (uint32_t)sizeof(T), r, sizeof(r));
+  uint32_t at = c.col * (uint32_t)sizeof(T);
+  asm volatile("" : "+v"(at));
+  if (c.live()) __builtin_memcpy(p + at, r, sizeof(r));
 }
 
 // a per-channel vector (fp32 or TH), or a constant
@@ -392,11 +397,11 @@ constexpr int SUMS = 4;
 // read from LDS (K = 1), where a workgroup puts them once.  16384 x 4096
 // bf16, gated: 220 us, 4.9 TB/s (321 us with twice the instructions and the
 // weights from L2).  Above 8192 columns (K = 2) the registers do not suffice
-// for two vectors a thread, and some are spilled: 2048 x 16384 283 us, 1.9
+// for two vectors a thread, and some are spilled: 2048 x 16384 194 us, 2.8
 // TB/s.
 template <typename TX, typename TH, int NT, int K, int V, bool LAYER>
 __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT,
-                             NT < WAVE || (LAYER && NT < 1024) ? 3 : 4) void
+                             LAYER && NT < 1024 ? 3 : 4) void
 norm_bwd_kernel(const NormArgs a, const NormGrads o) {
   constexpr int GROUPS = NT < BLOCK ? BLOCK / NT : 1;
   constexpr bool KEEP = K == 1;
@@ -772,11 +777,12 @@ extern "C" int launch_norm_fwd(void* stream, const NormArgs* a) {
   return go_types((hipStream_t)stream, *a, nullptr, 0);
 }
 
-// Workgroups of the backward pass: as many as the registers let a CU hold
-// (256 CUs: 1 of 1024 threads, 2 of 512, 4 of 256, with a LayerNorm 1, 1 and
-// 3), since each writes its column sums once; beyond 512 only where each still
-// has 8 turns.  16384 x 2048 bf16 RMSNorms: 512 workgroups take 118 us, 1024
-// take 112; fp32 and bf16 LayerNorms: 512 take 127, 768 133, 1024 155 us.
+// Workgroups of the backward pass: enough to fill 256 CUs, and no more, since
+// each writes its column sums once: one a CU of 1024 threads, 2 of 512, and up
+// to 4 of 256 where each still has 8 turns.  Half of that with LayerNorms,
+// whose four sums weigh more.  16384 x 2048 bf16 RMSNorms: 512 workgroups take
+// 118 us, 1024 take 112; fp32 and bf16 LayerNorms 124 and 131; 8192 x 4096 of
+// those 149 us with 256 and 157 with 512, the sums' addition included.
 extern "C" int norm_bwd_blocks(const NormArgs* a) {
   const int64_t groups = a->width <= 64    ? 32
                          : a->width <= 128 ? 16
@@ -788,7 +794,7 @@ extern "C" int norm_bwd_blocks(const NormArgs* a) {
   const int64_t turns = (a->rows + groups - 1) / groups;
   int64_t most = 512;
   if (a->width > 4096 || (layer && a->width > 2048)) most = 256;
-  else if (!layer && a->width <= 2048)
+  else if (a->width <= 2048 && !layer)
     most = std::min<int64_t>(std::max<int64_t>(512, turns / 8), 1024);
   return (int)std::min(turns, most);
 }
