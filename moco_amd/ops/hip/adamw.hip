@@ -450,17 +450,21 @@ __global__ __launch_bounds__(THREADS) void sumsq_kernel(
     partial[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-__global__ __launch_bounds__(THREADS) void norm_final_kernel(
+// (1024 threads: a launch's 2048 partial sums at most are two loads a thread)
+__global__ __launch_bounds__(1024) void norm_final_kernel(
     const double* __restrict__ partial, int n, float* __restrict__ out) {
   double acc = 0.0;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < n; i += THREADS) acc += partial[i];
+#pragma unroll 2
+  for (int i = threadIdx.x; i < n; i += 1024) acc += partial[i];
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, WAVE);
-  __shared__ double part[THREADS / WAVE];
+  __shared__ double part[1024 / WAVE];
   if (threadIdx.x % WAVE == 0) part[threadIdx.x / WAVE] = acc;
   __syncthreads();
-  if (threadIdx.x == 0)
-    *out = (float)sqrt((part[0] + part[1]) + (part[2] + part[3]));
+  if (threadIdx.x != 0) return;
+  acc = 0.0;
+#pragma unroll
+  for (int i = 0; i < 1024 / WAVE; ++i) acc += part[i];
+  *out = (float)sqrt(acc);
 }
 
 template <typename T>
@@ -544,8 +548,8 @@ extern "C" int launch_sumsq(void* stream, const GradTable* tab, int dtype,
 
 extern "C" int launch_norm_final(void* stream, const double* partial, int n,
                                  float* out) {
-  norm_final_kernel<<<dim3(1), THREADS, 0, (hipStream_t)stream>>>(partial, n,
-                                                                  out);
+  norm_final_kernel<<<dim3(1), 1024, 0, (hipStream_t)stream>>>(partial, n,
+                                                               out);
   HIP_CHECK_LAST();
   return 0;
 }
