@@ -155,7 +155,7 @@ def norm_residual(x: torch.Tensor, branch: Optional[torch.Tensor] = None, *,
                              "without one")
     scale_value = 1.0
     if isinstance(scale, torch.Tensor):
-        if scale.numel() == 1 and width > 1:
+        if scale.numel() == 1 and scale.shape != (width,):
             scale = scale.reshape(1).expand(width)
     elif scale is not None:
         scale, scale_value = None, float(scale)

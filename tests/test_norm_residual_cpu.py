@@ -157,7 +157,10 @@ def test_one_element_scale_and_no_affine():
     assert y is None and torch.allclose(r, x + 0.25 * m(h), atol=1e-6)
     r.sum().backward()
     assert torch.allclose(s.grad, m(h).sum().view(1), atol=1e-4)
-    assert norm_residual(x, h, scale=torch.tensor(0.5))[0].shape == x.shape
+    for shape in ((4, 32), (4, 1)):
+        r = norm_residual(torch.zeros(shape), torch.ones(shape),
+                          scale=torch.tensor(0.5))[0]
+        assert torch.equal(r, torch.full(shape, 0.5))
 
 
 def test_no_rows():

@@ -178,6 +178,20 @@ def test_one_module_for_both_norms_and_one_element_scale():
     assert torch.allclose(s.grad.double().cpu(), s2.grad, atol=0.1)
 
 
+def test_one_element_scale_of_any_shape():
+    from moco_amd.ops import norm_residual
+    for shape in ((4, 32), (4, 1)):
+        for s in (torch.tensor(0.5), torch.tensor([0.5]),
+                  torch.tensor([[0.5]])):
+            s = s.cuda().requires_grad_()
+            r = norm_residual(torch.zeros(shape, device="cuda"),
+                              torch.ones(shape, device="cuda"), scale=s)[0]
+            assert torch.equal(r, torch.full_like(r, 0.5))
+            r.sum().backward()
+            assert s.grad.shape == s.shape
+            assert float(s.grad) == r.numel()
+
+
 def run_graph(x, h, post, pre, leaves, d):
     from moco_amd.ops import norm_residual
     r, y = norm_residual(x, h, post=post, pre=pre, scale=0.5)
