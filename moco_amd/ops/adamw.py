@@ -192,7 +192,6 @@ def _decode(m: torch.Tensor, v: torch.Tensor, scales: torch.Tensor):
 # functional forms
 # ---------------------------------------------------------------------------
 
-@torch.no_grad()
 def grad_norm(grads: Tensors) -> torch.Tensor:
     """2-norm over all elements of all tensors, as a float32 scalar on their
     device (no host sync).  Squares and sums are taken in 64 bits.
@@ -213,21 +212,13 @@ def grad_norm(grads: Tensors) -> torch.Tensor:
                             f"got {g.dtype}")
         if g.device != grads[0].device:
             raise ValueError("gradients must be on one device")
-    return torch.stack([g.double().square().sum() for g in grads]
-                       ).sum().sqrt().float()
+    with torch.no_grad():
+        return torch.stack([g.double().square().sum() for g in grads]
+                           ).sum().sqrt().float()
 
 
-def _adamw(params, grads, ms, vs, scales, step, lr, betas, eps, weight_decay,
-           max_norm, total_norm, seed):
-    _check_step(step, lr, betas, eps, weight_decay, max_norm, total_norm)
-    params, grads = list(params), list(grads)
-    if use_hip(*params[:1]):
-        return ext().adamw_step(
-            params, grads, ms, vs, scales, int(step), lr, betas[0], betas[1],
-            eps, weight_decay, max_norm, total_norm, seed & 0xFFFFFFFF)
-    _check_lists(params, grads, ms, vs, scales)
-    if not params:
-        return total_norm
+def _plain_step(params, grads, ms, vs, scales, step, lr, betas, eps,
+                weight_decay, max_norm, total_norm, seed):
     coef = None
     if max_norm is not None:
         if total_norm is None:
@@ -267,7 +258,22 @@ def _adamw(params, grads, ms, vs, scales, step, lr, betas, eps, weight_decay,
     return total_norm
 
 
-@torch.no_grad()
+def _adamw(params, grads, ms, vs, scales, step, lr, betas, eps, weight_decay,
+           max_norm, total_norm, seed):
+    _check_step(step, lr, betas, eps, weight_decay, max_norm, total_norm)
+    params, grads = list(params), list(grads)
+    if use_hip(*params[:1]):
+        return ext().adamw_step(
+            params, grads, ms, vs, scales, int(step), lr, betas[0], betas[1],
+            eps, weight_decay, max_norm, total_norm, seed & 0xFFFFFFFF)
+    _check_lists(params, grads, ms, vs, scales)
+    if not params:
+        return total_norm
+    with torch.no_grad():
+        return _plain_step(params, grads, ms, vs, scales, step, lr, betas,
+                           eps, weight_decay, max_norm, total_norm, seed)
+
+
 def adamw_(params: Tensors, grads: Tensors, exp_avgs: Tensors,
            exp_avg_sqs: Tensors, *, step: int, lr: float,
            betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -293,7 +299,6 @@ def adamw_(params: Tensors, grads: Tensors, exp_avgs: Tensors,
                   eps, weight_decay, max_norm, total_norm, 0)
 
 
-@torch.no_grad()
 def adamw8bit_(params: Tensors, grads: Tensors, exp_avgs: Tensors,
                exp_avg_sqs: Tensors, scales: Tensors, *, step: int, lr: float,
                betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -311,7 +316,6 @@ def adamw8bit_(params: Tensors, grads: Tensors, exp_avgs: Tensors,
                   betas, eps, weight_decay, max_norm, total_norm, seed)
 
 
-@torch.no_grad()
 def adamw8bit_values(exp_avgs: Tensors, exp_avg_sqs: Tensors, scales: Tensors,
                      dtype: torch.dtype = torch.float32
                      ) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
@@ -335,11 +339,12 @@ def adamw8bit_values(exp_avgs: Tensors, exp_avg_sqs: Tensors, scales: Tensors,
         _check_scales(sc, m, i)
     ms, vs = [], []
     for m, v, s in zip(exp_avgs, exp_avg_sqs, scales):
-        mf, r = _decode(m, v, s)
-        for out, flat in ((ms, mf), (vs, r * r)):
-            t = torch.empty_like(m, dtype=dtype)
-            _flat(t).copy_(flat)
-            out.append(t)
+        with torch.no_grad():
+            mf, r = _decode(m, v, s)
+            for out, flat in ((ms, mf), (vs, r * r)):
+                t = torch.empty_like(m, dtype=dtype)
+                _flat(t).copy_(flat)
+                out.append(t)
     return ms, vs
 
 
