@@ -8,11 +8,12 @@
 //   p' = p (1 - lr wd)
 //        - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
-// Each operation is rounded by itself (no contraction into fma), as a plain
-// elementwise program in 32 bits does, and the root is rounded correctly, so
-// that what is rounded to 8 bits afterwards falls on the same codes (a root
-// that is off by an ulp moves one code in 2e5, and with it later steps).  The
-// reciprocal, which reaches the weights alone, is the hardware's: an ulp.
+// m' and v' are rounded operation by operation (no contraction into fma), as
+// a plain elementwise program in 32 bits does, and the root is rounded
+// correctly, so that what is rounded to 8 bits afterwards falls on the same
+// codes (a root that is off by an ulp moves one code in 2e5, and with it later
+// steps).  What reaches the weights alone takes the hardware's reciprocal, off
+// by an ulp at most, and fma.
 #include "common.h"
 #include "launchers.h"
 
@@ -112,6 +113,20 @@ __device__ __forceinline__ float clip_coef(const float* norm,
   return c > 1.f ? 1.f : c;
 }
 
+// The square root, rounded correctly: the hardware's is off by an ulp at most,
+// so it is that, or its neighbour below or above, by the signs of v - r r' for
+// the neighbours r'.  (A zero, an infinity and a NaN compare false.)  Below
+// 2^-96 the differences leave the normal range; there the hardware's stands.
+// Half of the instructions of sqrtf, which scales such values first.
+__device__ __forceinline__ float root(float v) {
+  const float r = __builtin_amdgcn_sqrtf(v);
+  const float below = __uint_as_float(__float_as_uint(r) - 1u);
+  const float above = __uint_as_float(__float_as_uint(r) + 1u);
+  float s = fmaf(-below, r, v) <= 0.f ? below : r;
+  s = fmaf(-above, r, v) > 0.f ? above : s;
+  return v < 0x1p-96f ? r : s;
+}
+
 // one element; r is sqrt(v')
 __device__ __forceinline__ void adamw_element(const AdamwScalars& h,
                                               float coef, float g, float& p,
@@ -119,9 +134,10 @@ __device__ __forceinline__ void adamw_element(const AdamwScalars& h,
   g = g * coef;
   m = m * h.beta1 + g * h.one_minus_beta1;
   v = v * h.beta2 + (g * g) * h.one_minus_beta2;
-  r = sqrtf(v);
-  const float q = m * __builtin_amdgcn_rcpf(r * h.inv_root_bc2 + h.eps);
-  p = p * h.decay - q * h.step_size;
+  r = root(v);
+  // what reaches the weights alone
+  const float q = m * __builtin_amdgcn_rcpf(fmaf(r, h.inv_root_bc2, h.eps));
+  p = fmaf(-q, h.step_size, p * h.decay);
 }
 
 // 28 bytes an fp32 element (22 a 16-bit one) and some 30 operations: bound
@@ -201,7 +217,7 @@ __device__ __forceinline__ float decode_root(uint32_t code) {
 
 __device__ __forceinline__ uint32_t encode_root(float q, uint32_t dither) {
   const uint32_t c = (__float_as_uint(q * 0x1p-112f) + dither) >> 19;
-  return q > 0.f ? min(max(c, 1u), 255u) : 0u;
+  return min(max(c, min(__float_as_uint(q), 1u)), 255u);  // 1 if q > 0
 }
 
 // 19 random bits of one element: a multiplicative hash of its counter (the
@@ -339,7 +355,7 @@ __global__ __launch_bounds__(THREADS) void adamw8_kernel(
       mf[j][k] *= s.x;
       adamw_element(h, coef, gf[j][k], pf[j][k], mf[j][k], v2, rf[j][k]);
       top_m = max(top_m, __float_as_uint(mf[j][k]) & 0x7FFFFFFFu);
-      top_r = max(top_r, __float_as_uint(rf[j][k]) & 0x7FFFFFFFu);
+      top_r = max(top_r, __float_as_uint(rf[j][k]));
     }
   }
   float sm = __uint_as_float(max16(top_m)) * (float)(1.0 / 448.0);
