@@ -386,20 +386,41 @@ struct TableFiller {
 torch::Tensor grad_norm_checked(const Refs& grads, bool again) {
   auto opts = grads[0].options().dtype(torch::kFloat32).layout(torch::kStrided);
   auto out = torch::empty({}, opts);
+  int64_t chunks_in_all = 0, bytes = 0;
+  int types = 0;  // a bit for each
+  uint16_t tail;
+  for (const auto* g : grads.t) {
+    if (!g->numel()) continue;
+    chunks_in_all += chunks_of(g->numel(), tail);
+    bytes += g->nbytes();
+    types |= 1 << adamw_dtype(*g, "gradients");
+  }
+  auto add = [&tail](GradTable& tab, const torch::Tensor& g, const auto& go) {
+    const int64_t chunks = chunks_of(g.numel(), tail);
+    const int i = next_slot(tab, GRAD_TENSORS, chunks, go);
+    tab.g[i] = g.const_data_ptr(), tab.tail[i] = tail;
+  };
+  if (chunks_in_all <= NORM_SMALL_CHUNKS && (types & (types - 1)) == 0) {
+    GradTable tab;
+    tab.count = 0, tab.chunks = 0;
+    for (const auto* g : grads.t)
+      if (g->numel()) add(tab, *g, [](const GradTable&) {});
+    CHECK_LAUNCH(launch_norm_small(cur_stream(), &tab, types / 2,
+                                   out.data_ptr<float>()));
+    return out;
+  }
   // workgroups of a launch at most: 8 per CU, which fill it with loads
   constexpr int64_t BLOCKS = 2048;
-  // a launch takes GRAD_TENSORS tensors of one dtype or MOST_CHUNKS chunks
-  int64_t launches = (int64_t)grads.size() / GRAD_TENSORS + 3, elements = 0;
-  int64_t bytes = 0;
-  for (const auto* g : grads.t) elements += g->numel(), bytes += g->nbytes();
   const bool once = !again && bytes > LAST_LEVEL_CACHE;
-  launches += 2 * (elements / ADAMW_CHUNK + (int64_t)grads.size()) /
-              MOST_CHUNKS;
+  // a launch takes GRAD_TENSORS tensors of one dtype or MOST_CHUNKS chunks
+  const int64_t launches = (int64_t)grads.size() / GRAD_TENSORS + 3 +
+                           2 * chunks_in_all / MOST_CHUNKS;
   auto partial = torch::empty({launches * BLOCKS},
                               opts.dtype(torch::kFloat64));
   double* at = partial.data_ptr<double>();
   int64_t used = 0;
   for (int dtype = 0; dtype < 3; ++dtype) {
+    if (!(types >> dtype & 1)) continue;
     auto go = [&](const GradTable& tab) {
       // as many as give each the same number of chunks
       const int64_t each = (tab.chunks + BLOCKS - 1) / BLOCKS;
@@ -411,13 +432,9 @@ torch::Tensor grad_norm_checked(const Refs& grads, bool again) {
     };
     GradTable tab;
     tab.count = 0, tab.chunks = 0;
-    for (const auto* g : grads.t) {
-      if (!g->numel() || adamw_dtype(*g, "gradients") != dtype) continue;
-      uint16_t tail;
-      const int64_t chunks = chunks_of(g->numel(), tail);
-      const int i = next_slot(tab, GRAD_TENSORS, chunks, go);
-      tab.g[i] = g->const_data_ptr(), tab.tail[i] = tail;
-    }
+    for (const auto* g : grads.t)
+      if (g->numel() && adamw_dtype(*g, "gradients") == dtype)
+        add(tab, *g, go);
     if (tab.count) go(tab);
   }
   CHECK_LAUNCH(launch_norm_final(cur_stream(), at, (int)used,

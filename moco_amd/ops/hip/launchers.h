@@ -102,6 +102,10 @@ int launch_adamw8_values(void* stream, const AdamwTable* tab, int dtype);
 // partial[blocks]: sums of squares of the table's g
 int launch_sumsq(void* stream, const GradTable* tab, int dtype,
                  double* partial, int blocks, bool once);
+// out = 2-norm of the table's g, of NORM_SMALL_CHUNKS chunks at most
+#define NORM_SMALL_CHUNKS 32
+int launch_norm_small(void* stream, const GradTable* tab, int dtype,
+                      float* out);
 // out = sqrt(sum of partial[0..n))
 int launch_norm_final(void* stream, const double* partial, int n, float* out);
 

@@ -213,7 +213,10 @@ def test_codes_are_those_of_32_bit_arithmetic():
 @pytest.mark.parametrize("dtype", list(HALF))
 def test_grad_norm_gpu(dtype):
     from moco_amd.ops import grad_norm
-    for shapes in (SHAPES, MANY, [(0,)], [(5_000_003,)]):
+    # one launch up to 32 chunks of 4096, two and more behind
+    for shapes in (SHAPES, MANY, [(0,)], [(5_000_003,)], [(1,)], [(4096,)],
+                   [(4097,), (0,), (3,)], [(131072,)], [(131073,)],
+                   [(5,)] * 32, [(5,)] * 33, [(4096,)] * 31 + [(4095,)]):
         gs = grads_for([torch.empty(s, dtype=dtype) for s in shapes], 3)
         want = np.sqrt(sum((mem(g) ** 2).sum() for g in gs))
         got = grad_norm(gs)
