@@ -459,14 +459,16 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Also takes the state of torch.optim.AdamW.  The moments keep their
-        own types (the base class casts them to the parameter's) and follow
-        their parameter's memory format."""
+        own types (the base class casts them to the parameter's, and a group
+        may so go on with 32-bit moments that were saved, whatever its
+        state_bits) and follow their parameter's memory format."""
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("amsgrad and maximize are not supported")
+        bits = [group["state_bits"] for group in self.param_groups]
         super().load_state_dict(state_dict)
-        for group in self.param_groups:
-            group.setdefault("state_bits", 32)
+        for group, own_bits in zip(self.param_groups, bits):
+            group.setdefault("state_bits", own_bits)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):

@@ -398,14 +398,17 @@ def test_optimizer_resumes_bit_for_bit(bits, dtype, tmp_path):
                 t.dtype == u.dtype and torch.equal(t.float(), u.float()))
 
 
-def test_optimizer_takes_state_of_torch_adamw():
+@pytest.mark.parametrize("bits", [8, 32])
+def test_optimizer_takes_state_of_torch_adamw(bits):
     a, b = params(), params()
     ob = torch.optim.AdamW(b, lr=0.01)
     give_grads(b, 0)
     ob.step()
     a = [torch.nn.Parameter(p.detach().clone()) for p in b]
-    oa = FusedAdamW(a, lr=0.3)
+    oa = FusedAdamW(a, lr=0.3, state_bits=bits)
     oa.load_state_dict(copy.deepcopy(ob.state_dict()))
+    assert oa.param_groups[0]["state_bits"] == bits
+    assert all(s["exp_avg"].dtype == torch.float32 for s in oa.state.values())
     give_grads(a, 1)
     give_grads(b, 1)
     oa.step()
