@@ -3,13 +3,16 @@
 // the C ABI of hip/launchers.h.
 #include <torch/extension.h>
 
+#include <ATen/FuncTorchTLS.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
 #include <array>
@@ -750,6 +753,7 @@ std::array<torch::Tensor, 3> norm_residual_fwd(
     bool want_stats) {
   TORCH_CHECK_VALUE(x.is_cuda(), "x must be a GPU tensor");
   at::cuda::CUDAGuard guard(x.device());
+  at::NoGradGuard no_grad;  // copies of strided inputs need no graph
   NormCall c(x, h, gate, w1, b1, w2, b2, scale, num.scale_value, num.post,
              num.pre, num.act, num.post_eps, num.pre_eps, (int)num.type_y);
   std::array<torch::Tensor, 3> out;
@@ -842,69 +846,56 @@ std::vector<torch::Tensor> norm_residual_bwd(
   return out;
 }
 
-class NormResidual : public torch::autograd::Function<NormResidual> {
- public:
-  // {r, y}, those that there are
-  static torch::autograd::variable_list forward(
-      torch::autograd::AutogradContext* ctx, const torch::Tensor& x,
-      const OptTensor& h, const OptTensor& gate, const OptTensor& w1,
-      const OptTensor& b1, const OptTensor& w2, const OptTensor& b2,
-      const OptTensor& scale, double scale_value, int64_t post, int64_t pre,
-      int64_t act, double post_eps, double pre_eps, int64_t type_y) {
-    const NormNumbers num{scale_value, post_eps, pre_eps, post,
-                          pre,         act,      type_y};
-    auto out = norm_residual_fwd(x, h, gate, w1, b1, w2, b2, scale, num, true);
-    const OptTensor* rest[7] = {&h, &gate, &w1, &b1, &w2, &b2, &scale};
-    torch::autograd::variable_list keep{x};
-    for (auto* t : rest) keep.push_back(t->value_or(torch::Tensor()));
-    keep.push_back(out[2]);
-    ctx->save_for_backward(keep);
-    ctx->saved_data["numbers"] =
-        std::vector<double>{scale_value,  post_eps,    pre_eps,
-                            (double)post, (double)pre, (double)act,
-                            (double)type_y};
-    ctx->set_materialize_grads(false);
-    torch::autograd::variable_list result;
-    for (int i = 0; i < 2; ++i)
-      if (out[i].defined()) result.push_back(out[i]);
-    return result;
+// The autograd node of a call.  (A Node, and not a torch::autograd::Function,
+// which wraps every argument and keeps what is no tensor in a dictionary:
+// 256 x 2048 both ways takes 105 us against 112.)
+struct NormResidualBackward : public torch::autograd::Node {
+  // x, branch, gate, post's weight and bias, pre's, scale
+  std::array<torch::autograd::SavedVariable, 8> saved;
+  torch::Tensor stats;
+  NormNumbers num;
+  bool has_r = false, has_y = false;
+
+  std::string name() const override { return "NormResidualBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& s : saved) s.reset_data();
+    stats.reset();
   }
 
-  static torch::autograd::variable_list backward(
-      torch::autograd::AutogradContext* ctx,
-      torch::autograd::variable_list grads) {
-    torch::autograd::variable_list result(15);
-    const auto saved = ctx->get_saved_variables();
-    const auto n = ctx->saved_data["numbers"].toDoubleVector();
-    const NormNumbers num{n[0],          n[1],          n[2],
-                          (int64_t)n[3], (int64_t)n[4], (int64_t)n[5],
-                          (int64_t)n[6]};
-    auto opt = [](const torch::Tensor& t) {
-      return t.defined() ? OptTensor(t) : OptTensor();
+  torch::autograd::variable_list apply(
+      torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    TORCH_CHECK(stats.defined(), torch::autograd::ERR_BACKWARD_TWICE);
+    torch::Tensor t[8];
+    bool again = false;  // a graph of the backward pass is asked for
+    for (int i = 0; i < 8; ++i) {
+      t[i] = saved[i].unpack();
+      again |= t[i].defined() && t[i].requires_grad();
+    }
+    for (const auto& g : grads) again |= g.defined() && g.requires_grad();
+    auto opt = [](const torch::Tensor& v) {
+      return v.defined() ? OptTensor(v) : OptTensor();
     };
     size_t at = 0;
     OptTensor d_r, d_y;
-    if (saved[1].defined()) d_r = opt(grads.at(at++));
-    if (num.pre != NORM_NONE) d_y = opt(grads.at(at++));
-    if (!d_r.has_value() && !d_y.has_value()) return result;
+    if (has_r) d_r = opt(grads.at(at++));
+    if (has_y) d_y = opt(grads.at(at++));
+    if (!d_r.has_value() && !d_y.has_value())
+      return torch::autograd::variable_list(8);
     int64_t want = 0;
-    size_t edge = 0;  // only tensors that are there have one
     for (int i = 0; i < 8; ++i)
-      if (saved[i].defined() && ctx->needs_input_grad(edge++)) want |= 1 << i;
-    auto out = norm_residual_bwd(
-        d_r, d_y, saved[8], saved[0], opt(saved[1]), opt(saved[2]),
-        opt(saved[3]), opt(saved[4]), opt(saved[5]), opt(saved[6]),
-        opt(saved[7]), num, want);
-    bool again = false;  // a graph of the backward pass is asked for
-    for (const auto& g : grads) again |= g.defined() && g.requires_grad();
-    for (const auto& v : saved) again |= v.defined() && v.requires_grad();
+      if (task_should_compute_output(i)) want |= 1 << i;
+    auto out = norm_residual_bwd(d_r, d_y, stats, t[0], opt(t[1]), opt(t[2]),
+                                 opt(t[3]), opt(t[4]), opt(t[5]), opt(t[6]),
+                                 opt(t[7]), num, want);
     if (again && at::GradMode::is_enabled()) {
       auto error = std::make_shared<torch::autograd::DelayedError>(
           "norm_residual has no second derivatives", (int64_t)out.size());
       out = (*error)(std::move(out));
     }
-    std::copy(out.begin(), out.end(), result.begin());
-    return result;
+    return out;
   }
 };
 
@@ -915,25 +906,40 @@ std::pair<OptTensor, OptTensor> norm_residual(
     const OptTensor& b2, const OptTensor& scale, double scale_value,
     int64_t post, int64_t pre, int64_t act, double post_eps, double pre_eps,
     int64_t type_y) {
-  bool train = x.requires_grad();
-  for (auto* t : {&h, &gate, &w1, &b1, &w2, &b2, &scale})
-    train |= t->has_value() && (*t)->requires_grad();
-  std::pair<OptTensor, OptTensor> out;
-  if (train && at::GradMode::is_enabled()) {
-    auto got = NormResidual::apply(x, h, gate, w1, b1, w2, b2, scale,
-                                   scale_value, post, pre, act, post_eps,
-                                   pre_eps, type_y);
-    size_t at = 0;
-    if (h.has_value()) out.first = got.at(at++);
-    if (pre != NORM_NONE) out.second = got.at(at++);
-  } else {
-    const NormNumbers num{scale_value, post_eps, pre_eps, post,
-                          pre,         act,      type_y};
-    auto got = norm_residual_fwd(x, h, gate, w1, b1, w2, b2, scale, num,
-                                 false);
-    if (got[0].defined()) out.first = got[0];
-    if (got[1].defined()) out.second = got[1];
+  if (const auto& func = at::functorch::functorchTLSAccessor())
+    func->checkSupportsCppAutogradFunction();
+  bool train = x.requires_grad(), tangent = x._fw_grad(0).defined();
+  for (auto* t : {&h, &gate, &w1, &b1, &w2, &b2, &scale}) {
+    if (!t->has_value()) continue;
+    train |= (*t)->requires_grad();
+    tangent |= (*t)->_fw_grad(0).defined();
   }
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !tangent, "norm_residual has no forward-mode derivatives on the GPU");
+  train = train && at::GradMode::is_enabled();
+  const NormNumbers num{scale_value, post_eps, pre_eps, post,
+                        pre,         act,      type_y};
+  auto got = norm_residual_fwd(x, h, gate, w1, b1, w2, b2, scale, num, train);
+  if (train) {
+    std::shared_ptr<NormResidualBackward> node(new NormResidualBackward(),
+                                               torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(
+        x, h, gate, w1, b1, w2, b2, scale));
+    node->saved[0] = torch::autograd::SavedVariable(x, false);
+    int i = 1;
+    for (auto* t : {&h, &gate, &w1, &b1, &w2, &b2, &scale})
+      node->saved[i++] =
+          torch::autograd::SavedVariable(t->value_or(torch::Tensor()), false);
+    node->stats = got[2];
+    node->num = num;
+    node->has_r = got[0].defined();
+    node->has_y = got[1].defined();
+    for (int k = 0; k < 2; ++k)
+      if (got[k].defined()) torch::autograd::set_history(got[k], node);
+  }
+  std::pair<OptTensor, OptTensor> out;
+  if (got[0].defined()) out.first = got[0];
+  if (got[1].defined()) out.second = got[1];
   return out;
 }
 

@@ -251,3 +251,66 @@ def test_refusals_gpu():
     (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_graph_of_a_call():
+    """What autograd promises for any node: two passes over a kept graph, an
+    error for a freed one and for an input changed in between, nothing for a
+    frozen input, the same under checkpointing and with half its outputs."""
+    from torch.utils.checkpoint import checkpoint
+
+    from moco_amd.ops import norm_residual
+    post, pre = (norms(k, 96, seed=i).cuda() for i, k in
+                 enumerate(("rms", "layer")))
+    gen = torch.Generator("cuda").manual_seed(5)
+    x, h, gate, d = (torch.randn(33, 96, device="cuda", generator=gen)
+                     for _ in range(4))
+    x.requires_grad_()
+    gate.requires_grad_()
+    leaves = [x, gate, *post.parameters(), *pre.parameters()]
+
+    def call(a, b, g):
+        return norm_residual(a, b, post=post, pre=pre, gate=g)
+
+    outs = call(x, h, gate)
+    assert all(o.requires_grad and o.grad_fn is not None for o in outs)
+    want = torch.autograd.grad(outs, leaves, (d, d), retain_graph=True)
+    again = torch.autograd.grad(outs, leaves, (d, d))
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(outs, leaves, (d, d))
+    got = torch.autograd.grad(checkpoint(call, x, h, gate,
+                                         use_reentrant=False), leaves, (d, d))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # one output only, the other's gradient absent or zero
+    some = torch.autograd.grad(call(x, h, gate)[1], leaves, d)
+    zero = torch.autograd.grad(call(x, h, gate), leaves,
+                               (torch.zeros_like(d), d))
+    assert all(torch.equal(a, b) for a, b in zip(some, zero))
+    # frozen inputs beside one that is not
+    y = call(x.detach(), h, gate.detach())[1]
+    y.backward(d)
+    assert h.grad is None and x.grad is None and gate.grad is None
+    assert all(p.grad is not None for p in pre.parameters())
+    outs = call(x, h, gate)
+    h.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(outs, leaves, (d, d))
+    with torch.no_grad():
+        assert not any(o.requires_grad for o in call(x, h, gate))
+
+
+def test_transforms_refused():
+    """Forward-mode tangents and function transforms are refused, not
+    dropped."""
+    import torch.autograd.forward_ad as fwAD
+
+    from moco_amd.ops import norm_residual
+    x, h, t = (torch.ones(2, 8, device="cuda") for _ in range(3))
+    with fwAD.dual_level():
+        for grad in (False, True):
+            dual = fwAD.make_dual(h.clone().requires_grad_(grad), t)
+            with pytest.raises(NotImplementedError):
+                norm_residual(x, dual)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: norm_residual(a, h)[0].sum())(x)
