@@ -465,6 +465,13 @@ class FusedAdamW(torch.optim.Optimizer):
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("amsgrad and maximize are not supported")
+            if not group.get("decoupled_weight_decay", True) and \
+                    group["weight_decay"]:
+                raise ValueError("the state's weight decay is Adam's, a part "
+                                 "of the gradient: not supported")
+        if any(not {"step", "exp_avg", "exp_avg_sq"} <= s.keys()
+               for s in state_dict["state"].values() if s):
+            raise ValueError("not the state of an AdamW: no step and moments")
         bits = [group["state_bits"] for group in self.param_groups]
         super().load_state_dict(state_dict)
         for group, own_bits in zip(self.param_groups, bits):

@@ -468,3 +468,22 @@ def test_optimizer_refusals():
     e(torch.tensor([1])).sum().backward()
     with pytest.raises(ValueError):
         FusedAdamW(e.parameters()).step()
+
+
+@pytest.mark.parametrize("other", [
+    lambda p: torch.optim.SGD(p, lr=0.1, momentum=0.9),
+    lambda p: torch.optim.Adam(p, lr=0.1, weight_decay=0.1)])
+def test_state_of_other_optimizers(other):
+    """Refused, with everything as it was."""
+    p = params()
+    before = other(p)
+    give_grads(p, 0)
+    before.step()
+    opt = FusedAdamW(p, lr=0.5)
+    opt.step()
+    kept = [opt.state[x]["exp_avg"].clone() for x in p]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(before.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5
+    assert all(torch.equal(opt.state[x]["exp_avg"], k)
+               for x, k in zip(p, kept))
