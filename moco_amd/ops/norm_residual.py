@@ -129,7 +129,8 @@ def norm_residual(x: torch.Tensor, branch: Optional[torch.Tensor] = None, *,
     before r is rounded to x's type.  Gradients flow to every tensor; x,
     branch and gate may be strided (halves of one projection) as long as the
     last dimension is dense, other layouts are copied.  On the GPU width is
-    16384 at most.
+    16384 at most, and only first derivatives of the backward kind are there:
+    second ones, forward-mode tangents and torch.func are errors.
     """
     width = x.shape[-1] if x.dim() else 0
     if width < 1:
