@@ -80,7 +80,9 @@ class MoCo(nn.Module):
         # hipGraph-replay-safe stepping (set by the engine): enqueue is
         # deferred to flush_queue() after backward (no queue snapshot
         # needed; ring ptr advanced on device), and at world size 1 the
-        # shuffling-BN exchange is skipped, as it is without a process group
+        # shuffling-BN exchange is skipped — a permutation is a no-op for
+        # batch statistics and is exactly inverted by the unshuffle, so
+        # single-rank semantics are unchanged (FP reduction order aside).
         self.graph_safe = False
         self._pending_keys: Optional[torch.Tensor] = None
 
@@ -159,12 +161,6 @@ class MoCo(nn.Module):
             step = self._step
             self._step += 1
         graph_safe = self.graph_safe and parallel.get_world_size() == 1
-        # One process keeps its key batch in order, eager or captured: batch
-        # statistics do not depend on a permutation, which the unshuffle
-        # inverts, but their rounding does.  Permuted, a ResNet-18 batch of 4
-        # differed by 1e-3 in its first loss from the captured step, and by
-        # 0.1 five steps later.
-        shuffle = not graph_safe and parallel.is_distributed()
         # the shuffle permutation is derived from (seed, step) on every rank
         # independently — verify the counters agree periodically (a desynced
         # rank would otherwise corrupt the key pairing SILENTLY)
@@ -174,7 +170,7 @@ class MoCo(nn.Module):
         with torch.no_grad():
             # start the key-batch exchange on the comm stream FIRST so the
             # xGMI transfer overlaps the query forward (join at key forward)
-            if shuffle:
+            if not graph_safe:
                 shuffle_job = parallel.begin_shuffle(im_k, step,
                                                      self.shuffle_seed)
             # EMA before the key forward, once per step (reference invariant)
@@ -190,8 +186,10 @@ class MoCo(nn.Module):
         q = l2_normalize(q, dim=1)
 
         with torch.no_grad():
-            if not shuffle:
-                # (nor would the host's per-step permutation be replay-safe)
+            if graph_safe:
+                # world-1 shuffle is exactly inverted by the unshuffle and
+                # batch statistics are permutation-invariant: skip it (the
+                # host-generated per-step permutation is not replay-safe)
                 k = self.encoder_k(im_k)
                 k = l2_normalize(k, dim=1)
             else:
