@@ -26,12 +26,22 @@ def _norm_args(mod: Optional[Norm], width: int, which: str):
     if mod is None:
         return 0, None, None, 0.0
     if isinstance(mod, nn.RMSNorm):
-        kind, bias = 1, None
+        kind, bias, base = 1, None, nn.RMSNorm
     elif isinstance(mod, nn.LayerNorm):
-        kind, bias = 2, mod.bias
+        kind, bias, base = 2, mod.bias, nn.LayerNorm
     else:
         raise TypeError(f"{which} must be an nn.RMSNorm or nn.LayerNorm, got "
                         f"{type(mod).__name__}")
+    # the formula is what the module itself would compute, and all it does
+    own = mod.__dict__
+    if "forward" in own or (type(mod) is not base and (
+            type(mod).forward is not base.forward or
+            type(mod).__call__ is not base.__call__)):
+        raise TypeError(f"{which}'s forward pass is not {base.__name__}'s: "
+                        f"{type(mod).__name__}")
+    if own["_forward_hooks"] or own["_forward_pre_hooks"] or \
+            own["_backward_hooks"] or own["_backward_pre_hooks"]:
+        raise TypeError(f"{which} has hooks, which would not be called")
     if mod.normalized_shape != (width,):
         raise ValueError(f"{which} normalizes {mod.normalized_shape}, the "
                          f"last dimension is {width}")
@@ -118,7 +128,9 @@ def norm_residual(x: torch.Tensor, branch: Optional[torch.Tensor] = None, *,
     x: [..., width], the residual stream; float32, or of the branch's type.
     branch: x's shape; float32, bfloat16 or float16, and the type of y.
     post, pre: nn.RMSNorm or nn.LayerNorm over the last dimension, with or
-        without weight and bias; None for no norm.
+        without weight and bias; None for no norm.  Only the formula is
+        computed and the module not called: one with hooks or with a forward
+        pass of its own is refused.
     gate: the branch's shape, or [..., 1] for one gate per token, of the
         branch's type; gate_act: None, "sigmoid" or "silu".
     scale: a number, or a tensor [width] (or of one element).  Weights,
