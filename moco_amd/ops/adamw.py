@@ -364,7 +364,8 @@ class FusedAdamW(torch.optim.Optimizer):
 
     All parameters lie on one device.  step() reads lr and the step count on
     the host, so it is not captured into a graph: run it after each replay,
-    as MoCoStepper does.
+    as MoCoStepper does.  state_dict() holds neither max_grad_norm nor seed,
+    which a resumed run gives again; copies and pickles of the optimizer do.
     """
 
     def __init__(self, params, lr: float = 1e-3,
@@ -378,6 +379,18 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps,
                                       weight_decay=weight_decay,
                                       state_bits=state_bits))
+
+    # the base class copies and pickles groups and state alone
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm,
+                "seed": self.seed, "last_grad_norm": self.last_grad_norm}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        # (a pickle of the base's part alone)
+        for name, value in (("max_grad_norm", None), ("seed", 0),
+                            ("last_grad_norm", None)):
+            self.__dict__.setdefault(name, value)
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)

@@ -1,0 +1,69 @@
+"""FusedAdamW survives copy.deepcopy and pickle."""
+
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+from moco_amd.ops import FusedAdamW
+
+
+def saved(opt):
+    f = io.BytesIO()
+    torch.save(opt, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)
+
+
+@pytest.mark.parametrize("device", [
+    "cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("clone", [
+    copy.deepcopy, saved, lambda o: pickle.loads(pickle.dumps(o))],
+    ids=["deepcopy", "save", "pickle"])
+@pytest.mark.parametrize("before", [0, 2])
+def test_copies_go_on_like_the_original(request, device, bits, clone, before):
+    if bits == 8 and before and "pickle" in request.node.name:
+        pytest.skip("pickle itself cannot read float8 tensors back")
+    torch.manual_seed(0)
+    ps = [torch.nn.Parameter(torch.randn(s, device=device))
+          for s in ((5, 7), (300,))]
+    opt = FusedAdamW(ps, lr=0.01, state_bits=bits, max_grad_norm=0.5, seed=9)
+    grads = [[torch.randn_like(p) for p in ps] for _ in range(before + 3)]
+
+    def step(o, gs):
+        for p, g in zip(o.param_groups[0]["params"], gs):
+            p.grad = g.clone()
+        o.step()
+
+    for gs in grads[:before]:
+        step(opt, gs)
+    other = clone(opt)
+    assert other.max_grad_norm == 0.5 and other.seed == 9
+    if before:
+        assert torch.equal(other.last_grad_norm, opt.last_grad_norm)
+    else:
+        assert other.last_grad_norm is None
+    for gs in grads[before:]:
+        step(opt, gs)
+        step(other, gs)
+    assert torch.equal(other.last_grad_norm, opt.last_grad_norm)
+    for p, q in zip(ps, other.param_groups[0]["params"]):
+        assert p is not q and torch.equal(p, q)
+        for k, t in opt.state[p].items():
+            u = other.state[q][k]
+            assert t == u if k == "step" else \
+                torch.equal(t.view(torch.uint8), u.view(torch.uint8))
+
+
+def test_loading_a_state_keeps_the_clip_and_the_seed():
+    p = torch.nn.Parameter(torch.randn(30))
+    p.grad = torch.randn(30)
+    opt = FusedAdamW([p], max_grad_norm=0.5, seed=9)
+    opt.step()
+    norm = opt.last_grad_norm
+    opt.load_state_dict(opt.state_dict())
+    assert (opt.max_grad_norm, opt.seed) == (0.5, 9)
+    assert opt.last_grad_norm is norm
