@@ -352,6 +352,35 @@ def adamw8bit_values(exp_avgs: Tensors, exp_avg_sqs: Tensors, scales: Tensors,
 # optimizer
 # ---------------------------------------------------------------------------
 
+def _check_saved(i: int, p: torch.Tensor, saved: dict) -> None:
+    """A parameter's saved state: moments of its shape, in 32 or 16 bits, or
+    codes with their scales."""
+    step = saved["step"]
+    if step is None or int(step) != step or step < 0:
+        raise ValueError(f"step of parameter {i} is {step}")
+    m, v = saved["exp_avg"], saved["exp_avg_sq"]
+    for t in (m, v):
+        if not isinstance(t, torch.Tensor) or t.layout != torch.strided or \
+                t.shape != p.shape:
+            raise ValueError(f"the moments of parameter {i} must be tensors "
+                             f"{tuple(p.shape)}")
+    scales = saved.get("scales")
+    if scales is None:
+        if m.dtype not in _FLOATS or v.dtype not in _FLOATS:
+            raise ValueError(f"the moments of parameter {i} are {m.dtype} and "
+                             f"{v.dtype}, without scales")
+        return
+    if m.dtype != torch.float8_e4m3fn or v.dtype != torch.uint8:
+        raise ValueError(f"the codes of parameter {i} are {m.dtype} and "
+                         f"{v.dtype}")
+    if not _is_dense(m) or not _same_layout(m, v):
+        raise ValueError(f"the codes of parameter {i} must be dense and laid "
+                         "out alike")
+    if not isinstance(scales, torch.Tensor):
+        raise ValueError(f"the scales of parameter {i} are not a tensor")
+    _check_scales(scales, m, i)
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """AdamW (torch.optim.AdamW's step) as a few fused HIP launches.
 
@@ -474,7 +503,8 @@ class FusedAdamW(torch.optim.Optimizer):
         """Also takes the state of torch.optim.AdamW.  The moments keep their
         own types (the base class casts them to the parameter's, and a group
         may so go on with 32-bit moments that were saved, whatever its
-        state_bits) and follow their parameter's memory format."""
+        state_bits) and follow their parameter's memory format.  A state that
+        does not fit is refused before anything is loaded."""
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("amsgrad and maximize are not supported")
@@ -485,14 +515,18 @@ class FusedAdamW(torch.optim.Optimizer):
         if any(not {"step", "exp_avg", "exp_avg_sq"} <= s.keys()
                for s in state_dict["state"].values() if s):
             raise ValueError("not the state of an AdamW: no step and moments")
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        states = [(i, p, state_dict["state"].get(i))
+                  for i, p in zip(ids, params)]
+        for i, p, saved in states:
+            if saved:
+                _check_saved(i, p, saved)
         bits = [group["state_bits"] for group in self.param_groups]
         super().load_state_dict(state_dict)
         for group, own_bits in zip(self.param_groups, bits):
             group.setdefault("state_bits", own_bits)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, params):
-            saved = state_dict["state"].get(i)
+        for _, p, saved in states:
             if not saved:
                 continue
             state = self.state[p]
