@@ -113,18 +113,23 @@ __device__ __forceinline__ float clip_coef(const float* norm,
   return c > 1.f ? 1.f : c;
 }
 
-// The square root, rounded correctly: the hardware's is off by an ulp at most,
-// so it is that, or its neighbour below or above, by the signs of v - r r' for
-// the neighbours r'.  (A zero, an infinity and a NaN compare false.)  Below
-// 2^-96 the differences leave the normal range; there the hardware's stands.
-// Half of the instructions of sqrtf, which scales such values first.
+// The square root, rounded correctly, of any v.  The hardware's is off by an
+// ulp at most for normal v (and zero for subnormal ones), so it is that, or its
+// neighbour below or above: by Tuckerman's test (Agarwal et al., "New scalar
+// and vector elementary functions for the IBM System/370", 1986), r is the root
+// rounded to nearest where r (r - ulp) < v <= r (r + ulp).  An fma gives those
+// differences' signs exactly where they are normal numbers, so a v below 2^-96
+// is scaled up first, by an even power of two.  (A zero, an infinity and a NaN
+// compare false.)
 __device__ __forceinline__ float root(float v) {
+  const bool small = v < 0x1p-96f;
+  v = small ? v * 0x1p96f : v;
   const float r = __builtin_amdgcn_sqrtf(v);
   const float below = __uint_as_float(__float_as_uint(r) - 1u);
   const float above = __uint_as_float(__float_as_uint(r) + 1u);
   float s = fmaf(-below, r, v) <= 0.f ? below : r;
   s = fmaf(-above, r, v) > 0.f ? above : s;
-  return v < 0x1p-96f ? r : s;
+  return small ? s * 0x1p-48f : s;
 }
 
 // one element; r is sqrt(v')
