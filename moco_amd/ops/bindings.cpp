@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <array>
@@ -255,6 +256,13 @@ void ema_flat(torch::Tensor dst, torch::Tensor src, double m) {
 
 using TensorList = std::vector<torch::Tensor>;
 
+// What these entry points launch goes past the dispatcher, so a tracer would
+// take their outputs for constants.
+void check_not_traced(const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), name,
+                              " cannot be traced on the GPU");
+}
+
 // The tensors of a Python list, borrowed: its items hold them during the
 // call (owning copies of 800 tensors cost as much time as all checks).
 struct Refs {
@@ -446,6 +454,7 @@ torch::Tensor grad_norm_checked(const Refs& grads, bool again) {
 }
 
 torch::Tensor grad_norm(const py::object& list, bool again) {
+  check_not_traced("grad_norm");
   Refs grads(list);
   TORCH_CHECK_VALUE(!grads.empty(), "grad_norm needs at least one tensor");
   const auto device = grads[0].device();
@@ -477,6 +486,7 @@ c10::optional<torch::Tensor> adamw_step(
     c10::optional<double> max_norm, c10::optional<torch::Tensor> total_norm,
     int64_t seed) {
   const bool eight = !scales_.is_none();
+  check_not_traced(eight ? "adamw8bit_" : "adamw_");
   const Refs params(params_), grads(grads_), ms(ms_), vs(vs_);
   const Refs scales = eight ? Refs(scales_) : Refs();
   const size_t n = params.size();
@@ -582,6 +592,7 @@ std::pair<TensorList, TensorList> adamw8bit_values(const py::object& ms_,
                                                    const py::object& vs_,
                                                    const py::object& scales_,
                                                    const py::object& dtype_) {
+  check_not_traced("adamw8bit_values");
   const Refs ms(ms_), vs(vs_), scales(scales_);
   const auto dtype = torch::python::detail::py_object_to_dtype(dtype_);
   TORCH_CHECK_VALUE(vs.size() == ms.size() && scales.size() == ms.size(),
@@ -908,6 +919,7 @@ std::pair<OptTensor, OptTensor> norm_residual(
     int64_t type_y) {
   if (const auto& func = at::functorch::functorchTLSAccessor())
     func->checkSupportsCppAutogradFunction();
+  check_not_traced("norm_residual");
   bool train = x.requires_grad(), tangent = x._fw_grad(0).defined();
   for (auto* t : {&h, &gate, &w1, &b1, &w2, &b2, &scale}) {
     if (!t->has_value()) continue;
