@@ -271,9 +271,14 @@ def _adamw(params, grads, ms, vs, scales, step, lr, betas, eps, weight_decay,
     _check_lists(params, grads, ms, vs, scales)
     if not params:
         return total_norm
+    # as the GPU's entry point takes them: a numpy or torch scalar would round
+    # what is computed of it to its own type
+    lr, eps, weight_decay = float(lr), float(eps), float(weight_decay)
+    betas = tuple(float(b) for b in betas)
+    max_norm = None if max_norm is None else float(max_norm)
     with torch.no_grad():
-        return _plain_step(params, grads, ms, vs, scales, step, lr, betas,
-                           eps, weight_decay, max_norm, total_norm, seed)
+        return _plain_step(params, grads, ms, vs, scales, int(step), lr, betas,
+                           eps, weight_decay, max_norm, total_norm, int(seed))
 
 
 def adamw_(params: Tensors, grads: Tensors, exp_avgs: Tensors,
