@@ -110,7 +110,7 @@ def _check_scales(s: torch.Tensor, like: torch.Tensor, i: int) -> None:
                          f"[{rows}, 2]")
 
 
-def _check_lists(params, grads, ms, vs, scales):
+def _check_lists(params, grads, ms, vs, scales, total_norm):
     n = len(params)
     if any(len(x) != n for x in (grads, ms, vs)) or \
             (scales is not None and len(scales) != n):
@@ -138,6 +138,12 @@ def _check_lists(params, grads, ms, vs, scales):
         if scales is not None:
             _check_scales(scales[i], p, i)
             spans.append((scales[i], True))
+    if params and total_norm is not None:
+        if total_norm.numel() != 1 or total_norm.dtype != torch.float32 \
+                or total_norm.device != params[0].device:
+            raise ValueError("total_norm must be one float32 on the tensors' "
+                             "device")
+        spans.append((total_norm, False))
     _check_overlap(spans)
 
 
@@ -225,10 +231,6 @@ def _plain_step(params, grads, ms, vs, scales, step, lr, betas, eps,
     if max_norm is not None:
         if total_norm is None:
             total_norm = grad_norm(grads)
-        elif total_norm.numel() != 1 or total_norm.dtype != torch.float32 \
-                or total_norm.device != params[0].device:
-            raise ValueError("total_norm must be one float32 on the tensors' "
-                             "device")
         coef = (torch.full_like(total_norm, max_norm)
                 / (total_norm + 1e-6)).clamp(max=1.0).reshape(())
     b1, b2 = betas
@@ -268,7 +270,7 @@ def _adamw(params, grads, ms, vs, scales, step, lr, betas, eps, weight_decay,
         return ext().adamw_step(
             params, grads, ms, vs, scales, int(step), lr, betas[0], betas[1],
             eps, weight_decay, max_norm, total_norm, seed & 0xFFFFFFFF)
-    _check_lists(params, grads, ms, vs, scales)
+    _check_lists(params, grads, ms, vs, scales, total_norm)
     if not params:
         return total_norm
     # as the GPU's entry point takes them: a numpy or torch scalar would round
@@ -292,8 +294,8 @@ def adamw_(params: Tensors, grads: Tensors, exp_avgs: Tensors,
     params, grads: float32, bfloat16 or float16, a gradient of its
         parameter's type; exp_avgs, exp_avg_sqs: float32.  The four of one
         parameter are dense and laid out alike (in any memory format), all on
-        one device, and no two tensors share memory (a gradient may be given
-        for several parameters).
+        one device, and what is written shares no memory (a gradient may be
+        given for several parameters).
     step: counts from 1.
     max_norm: scales the gradients (where they are used, not in memory) by
         min(1, max_norm / (norm + 1e-6)).  norm is `total_norm`, a float32

@@ -539,14 +539,17 @@ c10::optional<torch::Tensor> adamw_step(
   int64_t bytes = 0;
   for (const auto& r : ranges) bytes += r.end - r.begin;
   const bool once = bytes > LAST_LEVEL_CACHE;
-  check_disjoint(ranges);
-  const float* norm = nullptr;
-  if (max_norm.has_value()) {
-    if (!total_norm.has_value()) total_norm = grad_norm_checked(grads, true);
+  if (max_norm.has_value() && total_norm.has_value()) {
     TORCH_CHECK_VALUE(total_norm->device() == device &&
                           total_norm->numel() == 1 &&
                           total_norm->scalar_type() == torch::kFloat32,
                       "total_norm must be one float32 on the tensors' device");
+    add_range(ranges, *total_norm, false);
+  }
+  check_disjoint(ranges);
+  const float* norm = nullptr;
+  if (max_norm.has_value()) {
+    if (!total_norm.has_value()) total_norm = grad_norm_checked(grads, true);
     norm = total_norm->const_data_ptr<float>();
   }
   AdamwScalars h;

@@ -49,3 +49,36 @@ def test_numbers_of_any_type(device, eight, to):
     call(*b, step=3, betas=betas, **kw)
     for x, y in zip(a, b):
         assert torch.equal(x[0].view(torch.uint8), y[0].view(torch.uint8))
+
+
+@devices
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("which", [0, 2, 3, 4])
+def test_a_norm_among_what_is_written(device, eight, which):
+    """A workgroup might read it after another has written it."""
+    if which >= (5 if eight else 4):
+        return
+    call = adamw8bit_ if eight else adamw_
+    st = state(eight, device)
+    was = [x[0].clone() for x in st]
+    flat = st[which][0].view(-1).view(torch.uint8)
+    at = 8 if which == 4 else 256
+    norm = flat[at:at + 4].view(torch.float32)
+    with pytest.raises(ValueError):
+        call(*st, step=1, lr=0.1, max_norm=1.0, total_norm=norm)
+    for x, y in zip(was, st):
+        assert torch.equal(x.view(torch.uint8), y[0].view(torch.uint8))
+
+
+@devices
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_norm_among_the_gradients(device, eight):
+    """Only read, so allowed."""
+    call = adamw8bit_ if eight else adamw_
+    a, b = state(eight, device), state(eight, device)
+    norm = a[1][0][4]
+    out = call(*a, step=1, lr=0.1, max_norm=1.0, total_norm=norm)
+    call(*b, step=1, lr=0.1, max_norm=1.0, total_norm=norm.clone())
+    assert out is norm or torch.equal(out, norm)
+    for x, y in zip(a, b):
+        assert torch.equal(x[0].view(torch.uint8), y[0].view(torch.uint8))
