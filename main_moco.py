@@ -51,7 +51,8 @@ def get_parser():
     parser.add_argument("--optimizer", default="sgd",
                         choices=["sgd", "adamw", "adamw8bit"],
                         help="adamw8bit keeps AdamW's moments in 8 bits; "
-                             "--momentum is SGD's (AdamW: betas 0.9, 0.999)")
+                             "--momentum is SGD's (AdamW: betas 0.9, 0.999), "
+                             "and so is --lr's default")
     parser.add_argument("--clip-grad", default=None, type=float,
                         help="AdamW: clip the gradients' global norm to this")
     parser.add_argument("-p", "--print-freq", default=10, type=int)
@@ -104,6 +105,9 @@ def main(argv=None):
     args = parser.parse_args(argv)
     if args.clip_grad is not None and args.optimizer == "sgd":
         parser.error("--clip-grad needs --optimizer adamw or adamw8bit")
+    if args.optimizer != "sgd" and args.lr == parser.get_default("lr"):
+        warnings.warn(f"--lr {args.lr} is SGD's default; AdamW mostly takes "
+                      "1e-4 to 1e-3")
 
     if args.debug_serialize:
         # must be set before the first HIP call in every worker
