@@ -297,6 +297,18 @@ int adamw_dtype(const torch::Tensor& t, const char* what) {
                    t.scalar_type());
 }
 
+// whether a tensor's memory holds its values: not so where it is lazily negated
+// (the imaginary part of a conjugate), or a zero that has no memory
+bool in_memory(const torch::Tensor& t) {
+  return !t.is_neg() && !t._is_zerotensor();
+}
+
+// the values, without gaps
+torch::Tensor laid_out(const torch::Tensor& t) {
+  return in_memory(t) ? t.contiguous()
+                      : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // same shape and same place of every element (strides of length-1 dims say
 // nothing), without gaps
 bool same_dense_layout(const torch::Tensor& a, const torch::Tensor& b) {
@@ -470,8 +482,8 @@ torch::Tensor grad_norm(const py::object& list, bool again) {
     adamw_dtype(*g, "gradients");
     // an expanded or gapped view is laid out first: each element counts once
     // per place that it has in the tensor
-    if (g->is_non_overlapping_and_dense()) continue;
-    copies.push_back(g->contiguous());
+    if (g->is_non_overlapping_and_dense() && in_memory(*g)) continue;
+    copies.push_back(laid_out(*g));
     g = &copies.back();
   }
   return grad_norm_checked(grads, again);
@@ -519,6 +531,10 @@ c10::optional<torch::Tensor> adamw_step(
                           same_dense_layout(p, v),
                       "parameter ", i, ", its gradient and its moments must "
                       "be dense and laid out alike");
+    TORCH_CHECK_VALUE(in_memory(p) && in_memory(g) && in_memory(m) &&
+                          in_memory(v) && (!eight || in_memory(scales[i])),
+                      "a tensor of parameter ", i, " is lazily negated or a "
+                      "zero without memory");
     add_range(ranges, p, true);
     add_range(ranges, g, false);
     add_range(ranges, m, true);
@@ -541,7 +557,7 @@ c10::optional<torch::Tensor> adamw_step(
   const bool once = bytes > LAST_LEVEL_CACHE;
   if (max_norm.has_value() && total_norm.has_value()) {
     TORCH_CHECK_VALUE(total_norm->device() == device &&
-                          total_norm->numel() == 1 &&
+                          total_norm->numel() == 1 && in_memory(*total_norm) &&
                           total_norm->scalar_type() == torch::kFloat32,
                       "total_norm must be one float32 on the tensors' device");
     add_range(ranges, *total_norm, false);
@@ -620,6 +636,9 @@ std::pair<TensorList, TensorList> adamw8bit_values(const py::object& ms_,
                       "all tensors must be on one device");
     TORCH_CHECK_VALUE(same_dense_layout(m, v),
                       "codes ", i, " must be dense and laid out alike");
+    TORCH_CHECK_VALUE(in_memory(m) && in_memory(v) && in_memory(s),
+                      "codes ", i, " are lazily negated or zeros without "
+                      "memory");
     TORCH_CHECK_VALUE(s.scalar_type() == torch::kFloat32 &&
                           s.is_contiguous() && s.dim() == 2 &&
                           s.size(0) == (m.numel() + 255) / 256 &&
@@ -656,7 +675,7 @@ struct Rows {
   explicit Rows(const torch::Tensor& in) : t(in) {
     const int64_t width = in.size(-1);
     ld = width;
-    bool ok = width <= 1 || in.stride(-1) == 1;
+    bool ok = (width <= 1 || in.stride(-1) == 1) && in_memory(in);
     int64_t want = -1;  // stride that the next dimension outwards must have
     for (int64_t d = in.dim() - 2; ok && d >= 0; --d) {
       if (in.size(d) == 1) continue;
@@ -665,7 +684,7 @@ struct Rows {
       want = in.stride(d) * in.size(d);
     }
     if (!ok) {
-      t = in.contiguous();
+      t = laid_out(in);
       ld = width;
     }
   }
@@ -687,7 +706,7 @@ struct NormCall {
                      "scale must be float32 or of the block's type, got ",
                      v->scalar_type());
     if (type == 0) a.f32 |= 1 << bit;
-    keep.push_back(v->contiguous());
+    keep.push_back(laid_out(*v));
     return keep.back().const_data_ptr();
   }
 
@@ -809,13 +828,13 @@ std::vector<torch::Tensor> norm_residual_bwd(
     TORCH_CHECK(d_r->sizes() == x.sizes() &&
                 d_r->scalar_type() == x.scalar_type() &&
                 d_r->device() == x.device());
-    dr = d_r->contiguous();
+    dr = laid_out(*d_r);
     o.d_r = dr.const_data_ptr();
   }
   if (d_y.has_value()) {
     TORCH_CHECK(d_y->sizes() == x.sizes() && d_y->scalar_type() == type_h &&
                 d_y->device() == x.device() && num.pre != NORM_NONE);
-    dy = d_y->contiguous();
+    dy = laid_out(*d_y);
     o.d_y = dy.const_data_ptr();
   }
   std::vector<torch::Tensor> out(8);
