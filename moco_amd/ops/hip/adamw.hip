@@ -304,10 +304,11 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint2 w, int n) {
 // 16 lanes share a block of 256 elements: lane l holds elements l*8.. of
 // each half, so that a wave reads whole lines and the block's maximum needs
 // no shared memory (four DPP steps).  16 bytes an fp32 element (10 a 16-bit
-// one) against some 60 operations, which leaves the vector units little to
-// spare: with a correctly rounded root and quotient they were the limit (2e8
-// bf16 weights 430 us, with the hardware's 380, 5.3 TB/s).  Codes go through
-// the caches in any case: their next reader may find them there.
+// one) against some 65 operations, which leaves the vector units little to
+// spare: 2e8 bf16 weights 361 us, 5.6 TB/s, of which the root's scaling of
+// values below 2^-96 takes some 7; with the library's root and a rounded
+// quotient they were the limit, at 430.  Codes go through the caches in any
+// case: their next reader may find them there.
 template <typename T, bool ONCE>
 __global__ __launch_bounds__(THREADS) void adamw8_kernel(
     const AdamwTable tab, const AdamwScalars h, const float* norm,
@@ -431,8 +432,10 @@ __global__ __launch_bounds__(THREADS) void adamw8_values_kernel(
 
 // ---- gradient norm ---------------------------------------------------------
 // Squares and sums in 64 bits: a square of a 32-bit value is exact there,
-// and the order of the sum does not reach the 32-bit result.  Bound by
-// reading 4 (2) bytes an element: 300 MB in bf16 take 54 us, 5.6 TB/s.
+// and the order of the sum hardly ever reaches the 32-bit result (its value
+// would have to lie within some 2^-42 of a border between two).  The order is
+// that of the list, so the same list gives the same bits.  Bound by reading 4
+// (2) bytes an element: 300 MB in bf16 take 53 us, 5.7 TB/s.
 
 // root of the sum over a workgroup of 1024
 __device__ __forceinline__ void finish_norm(double acc, float* out) {

@@ -194,9 +194,11 @@ struct RowSum {
   }
 };
 
-// 1 / (1 + exp(-g)) by the hardware's exp2 and reciprocal: off by (2 + |g|) U
-// (the rounding of g log2(e), and an ulp each), an eighth of expf's and a
-// division's instructions
+// 1 / (1 + exp(-g)) by the hardware's exp2 and reciprocal: off by
+// (5 + 1.25 |g|) U of itself, U = 2^-24: an ulp (2U) each and U for the sum,
+// and g log2(e) is off by its rounding, U, and its constant's, 0.22 U, which
+// the exponential makes |g| times as much.  An eighth of expf's and a
+// division's instructions.
 __device__ __forceinline__ float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(
       1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f));
@@ -283,7 +285,8 @@ struct FwdRow {
 // weights in registers (K = 1) over its rows, and the next row's inputs are on
 // their way while this one's sums are taken.  16384 x 4096 bf16, gated: 125
 // us, 5.4 TB/s, where a copy of 4 GB reaches 4.75 (one row a workgroup, its
-// weights read each time: 170 us).
+// weights read each time: 170 us).  Above 8192 columns (K = 2) 4.0 TB/s; fp32
+// blocks spill 4 to 10 registers there.
 template <typename TX, typename TH, int NT, int K, int V, bool LAYER>
 __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT) void norm_fwd_kernel(
     const NormArgs a) {
@@ -395,10 +398,11 @@ constexpr int SUMS = 4;
 // and registers, which bound how many rows are on their way per CU.  So hats
 // and weighted values are made again rather than kept, and the weights are
 // read from LDS (K = 1), where a workgroup puts them once.  16384 x 4096
-// bf16, gated: 220 us, 4.9 TB/s (321 us with twice the instructions and the
+// bf16, gated: 205 us, 5.2 TB/s (321 us with twice the instructions and the
 // weights from L2).  Above 8192 columns (K = 2) the registers do not suffice
-// for two vectors a thread, and some are spilled: 2048 x 16384 194 us, 2.8
-// TB/s.
+// for two vectors a thread, and 44 to 306 are spilled: 2048 x 16384 194 us, 2.8
+// TB/s.  (Two LayerNorm forms under an fp32 stream spill one or two from 4097
+// columns on.)
 template <typename TX, typename TH, int NT, int K, int V, bool LAYER>
 __global__ __launch_bounds__(NT < BLOCK ? BLOCK : NT,
                              LAYER && NT < 1024 ? 3 : 4) void
