@@ -28,7 +28,8 @@ moves it by some 0.05%, codes are 3 to 6% apart, and rounding to nearest would
 hold it still.  A v above zero keeps a code above zero.  A gradient that is
 not finite reaches the scale, so all 256 elements of its block.
 
-On the GPU torch.jit.trace of these functions is an error.
+On the GPU torch.jit.trace and make_fx of these functions, and fake tensors,
+are errors.
 """
 
 import math

@@ -6,6 +6,7 @@
 #include <ATen/FuncTorchTLS.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <torch/csrc/autograd/function.h>
@@ -257,10 +258,25 @@ void ema_flat(torch::Tensor dst, torch::Tensor src, double m) {
 using TensorList = std::vector<torch::Tensor>;
 
 // What these entry points launch goes past the dispatcher, so a tracer would
-// take their outputs for constants.
+// take their outputs for constants; FakeTensorMode, make_fx and what is built
+// on them run through here with tensors of which there is only the shape.
 void check_not_traced(const char* name) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), name,
-                              " cannot be traced on the GPU");
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !torch::jit::tracer::isTracing() &&
+          !Modes::get_mode(Key::FAKE).has_value() &&
+          !Modes::get_mode(Key::PROXY).has_value() &&
+          !Modes::get_mode(Key::FUNCTIONAL).has_value(),
+      name, " cannot be traced on the GPU");
+}
+
+// A subclass that answers for itself when operators are called has no memory
+// of its own, and its data pointer may be null.
+void check_own_memory(const torch::Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python),
+      "a tensor subclass with its own dispatch has no memory for a kernel");
 }
 
 // The tensors of a Python list, borrowed: its items hold them during the
@@ -279,6 +295,7 @@ struct Refs {
       PyObject* x = PySequence_Fast_GET_ITEM(hold.ptr(), i);
       TORCH_CHECK_TYPE(THPVariable_Check(x), "a list of tensors is expected");
       t.push_back(&THPVariable_Unpack(x));
+      check_own_memory(*t.back());
     }
   }
   size_t size() const { return t.size(); }
@@ -499,6 +516,7 @@ c10::optional<torch::Tensor> adamw_step(
     int64_t seed) {
   const bool eight = !scales_.is_none();
   check_not_traced(eight ? "adamw8bit_" : "adamw_");
+  if (total_norm.has_value()) check_own_memory(*total_norm);
   const Refs params(params_), grads(grads_), ms(ms_), vs(vs_);
   const Refs scales = eight ? Refs(scales_) : Refs();
   const size_t n = params.size();
@@ -901,13 +919,20 @@ struct NormResidualBackward : public torch::autograd::Node {
       torch::autograd::variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     TORCH_CHECK(stats.defined(), torch::autograd::ERR_BACKWARD_TWICE);
+    check_not_traced("norm_residual's backward pass");
     torch::Tensor t[8];
     bool again = false;  // a graph of the backward pass is asked for
     for (int i = 0; i < 8; ++i) {
       t[i] = saved[i].unpack();
-      again |= t[i].defined() && t[i].requires_grad();
+      if (!t[i].defined()) continue;
+      check_own_memory(t[i]);
+      again |= t[i].requires_grad();
     }
-    for (const auto& g : grads) again |= g.defined() && g.requires_grad();
+    for (const auto& g : grads) {
+      if (!g.defined()) continue;
+      check_own_memory(g);
+      again |= g.requires_grad();
+    }
     auto opt = [](const torch::Tensor& v) {
       return v.defined() ? OptTensor(v) : OptTensor();
     };
@@ -942,9 +967,11 @@ std::pair<OptTensor, OptTensor> norm_residual(
   if (const auto& func = at::functorch::functorchTLSAccessor())
     func->checkSupportsCppAutogradFunction();
   check_not_traced("norm_residual");
+  check_own_memory(x);
   bool train = x.requires_grad(), tangent = x._fw_grad(0).defined();
   for (auto* t : {&h, &gate, &w1, &b1, &w2, &b2, &scale}) {
     if (!t->has_value()) continue;
+    check_own_memory(**t);
     train |= (*t)->requires_grad();
     tangent |= (*t)->_fw_grad(0).defined();
   }

@@ -142,8 +142,8 @@ def norm_residual(x: torch.Tensor, branch: Optional[torch.Tensor] = None, *,
     branch and gate may be strided (halves of one projection) as long as the
     last dimension is dense, other layouts are copied.  On the GPU width is
     16384 at most, and only first derivatives of the backward kind are there:
-    second ones, forward-mode tangents, torch.func and torch.jit.trace are
-    errors.
+    second ones, forward-mode tangents, torch.func, torch.jit.trace, make_fx
+    and fake tensors are errors.
     """
     width = x.shape[-1] if x.dim() else 0
     if width < 1:
