@@ -454,7 +454,7 @@ class FusedAdamW(torch.optim.Optimizer):
                                     else torch.float32)
         if bits == 8:
             state["scales"] = torch.zeros(-(-p.numel() // BLOCK), 2,
-                                          device=p.device)
+                                          dtype=torch.float32, device=p.device)
         return state
 
     @torch.no_grad()
