@@ -37,4 +37,5 @@ def test_default_dtype(device, bits, default):
         torch.set_default_dtype(old)
     for a, b in zip(want, got):
         assert a.dtype == b.dtype
-        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        assert torch.equal(a.reshape(-1).view(torch.uint8),
+                           b.reshape(-1).view(torch.uint8))
