@@ -1452,12 +1452,12 @@ torch::Tensor two_crop_augment(torch::Tensor src, torch::Tensor params,
     out = out.contiguous(torch::MemoryFormat::ChannelsLast);
   auto tmp1 = torch::empty({M, 3, S, S}, f32);
   auto tmp2 = torch::empty({M, 3, S, S}, f32);
-  auto graysum = torch::zeros({M}, f32);
+  auto graypart = torch::empty({M, (S * S + 255) / 256}, f32);
   CHECK_LAUNCH(launch_two_crop_augment(
       cur_stream(), src.data_ptr(),
       src.scalar_type() == torch::kUInt8, params.data_ptr<float>(),
       out.data_ptr(), tmp1.data_ptr<float>(), tmp2.data_ptr<float>(),
-      graysum.data_ptr<float>(), B, M, H, W, S, out_bf16, channels_last));
+      graypart.data_ptr<float>(), B, M, H, W, S, out_bf16, channels_last));
   return out;
 }
 

@@ -47,7 +47,7 @@ __device__ __forceinline__ float src_val<unsigned char>(unsigned char v) {
 template <typename ST>
 __global__ __launch_bounds__(256) void aug_crop_resize_kernel(
     const ST* __restrict__ src, const float* __restrict__ params,
-    float* __restrict__ tmp1, float* __restrict__ graysum, int B, int H,
+    float* __restrict__ tmp1, float* __restrict__ graypart, int B, int H,
     int W, int S) {
   const int m = blockIdx.y;
   const int p = blockIdx.x * 256 + threadIdx.x;
@@ -81,13 +81,16 @@ __global__ __launch_bounds__(256) void aug_crop_resize_kernel(
     }
     g_acc = gray_of(out3[0], out3[1], out3[2]);
   }
-  // block-reduce the gray contribution, one atomic per block
+  // block-reduce the gray contribution: one partial sum per block, which
+  // pass 2 adds in a fixed order (atomics would add them in any, and equal
+  // calls would differ)
   g_acc = wave_reduce_sum(g_acc);
   __shared__ float ws[4];
   if (threadIdx.x % WAVE == 0) ws[threadIdx.x / WAVE] = g_acc;
   __syncthreads();
   if (threadIdx.x == 0)
-    atomicAdd(&graysum[m], ws[0] + ws[1] + ws[2] + ws[3]);
+    graypart[(int64_t)m * gridDim.x + blockIdx.x] =
+        ws[0] + ws[1] + ws[2] + ws[3];
 }
 
 // ---- hue helpers (match ops/augment.py _rgb_to_hsv/_hsv_to_rgb) -----------
@@ -133,9 +136,18 @@ __device__ void hue_rotate(float& r, float& g, float& b, float dh) {
 // ---- pass 2: jitter + grayscale -------------------------------------------
 __global__ __launch_bounds__(256) void aug_jitter_kernel(
     const float* __restrict__ tmp1, const float* __restrict__ params,
-    const float* __restrict__ graysum, float* __restrict__ tmp2, int S) {
+    const float* __restrict__ graypart, float* __restrict__ tmp2, int S) {
   const int m = blockIdx.y;
   const int p = blockIdx.x * 256 + threadIdx.x;
+  // the crop's gray sum, of as many partial sums as this grid is wide
+  float part = 0.f;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256)
+    part += graypart[(int64_t)m * gridDim.x + i];
+  part = wave_reduce_sum(part);
+  __shared__ float ws[4];
+  if (threadIdx.x % WAVE == 0) ws[threadIdx.x / WAVE] = part;
+  __syncthreads();
+  const float graysum = ws[0] + ws[1] + ws[2] + ws[3];
   if (p >= S * S) return;
   const float* pm = params + m * 12;
   const int64_t base = (int64_t)m * 3 * S * S;
@@ -160,7 +172,7 @@ __global__ __launch_bounds__(256) void aug_jitter_kernel(
   // exact for unclipped pixels (documented approximation).
   const float co = pm[P_CO];
   const float mean_g =
-      __saturatef(graysum[m] / (float)(S * S) * br);
+      __saturatef(graysum / (float)(S * S) * br);
   r = __saturatef(co * r + (1.f - co) * mean_g);
   g = __saturatef(co * g + (1.f - co) * mean_g);
   b = __saturatef(co * b + (1.f - co) * mean_g);
@@ -266,21 +278,21 @@ __global__ __launch_bounds__(256) void aug_blur_v_finalize_kernel(
 extern "C" int launch_two_crop_augment(void* stream, const void* src,
                                        bool src_u8, const float* params,
                                        void* out, float* tmp1, float* tmp2,
-                                       float* graysum, int64_t B, int64_t M,
+                                       float* graypart, int64_t B, int64_t M,
                                        int64_t H, int64_t W, int64_t S,
                                        bool out_bf16, bool channels_last) {
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)((S * S + 255) / 256), (unsigned)M);
   if (src_u8)
     aug_crop_resize_kernel<unsigned char><<<grid, 256, 0, s>>>(
-        (const unsigned char*)src, params, tmp1, graysum, (int)B, (int)H,
+        (const unsigned char*)src, params, tmp1, graypart, (int)B, (int)H,
         (int)W, (int)S);
   else
     aug_crop_resize_kernel<float><<<grid, 256, 0, s>>>(
-        (const float*)src, params, tmp1, graysum, (int)B, (int)H, (int)W,
+        (const float*)src, params, tmp1, graypart, (int)B, (int)H, (int)W,
         (int)S);
   HIP_CHECK_LAST();
-  aug_jitter_kernel<<<grid, 256, 0, s>>>(tmp1, params, graysum, tmp2,
+  aug_jitter_kernel<<<grid, 256, 0, s>>>(tmp1, params, graypart, tmp2,
                                          (int)S);
   HIP_CHECK_LAST();
   aug_blur_h_kernel<<<grid, 256, 0, s>>>(tmp2, params, tmp1, (int)S);
